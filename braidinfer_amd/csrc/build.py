@@ -44,8 +44,10 @@ MODULES: Dict[str, List[str]] = {
     "routed_experts": ["routed_experts.hip"],
     "experts_wide": ["experts_wide.hip"],
     "streams": ["streams.hip"],
+    "kv4_cache": ["kv4_cache.hip"],
+    "attention_kv4": ["attention_kv4.hip"],
 }
-HEADERS = ["common.h", "no_alloc.h", "expert_units.h", "prefill_order.h"]
+HEADERS = ["common.h", "no_alloc.h", "expert_units.h", "prefill_order.h", "kv4.h"]
 
 _loaded: Dict[str, ctypes.CDLL] = {}
 _lock = threading.Lock()

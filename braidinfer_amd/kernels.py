@@ -1865,6 +1865,171 @@ def attention_decode_fuses_rope(hd: int, nq: int, nkv: int, page: int, table_pag
             and -(-table_pages // max(1, nsplit)) <= 1024)
 
 
+# ------------------------------------------------- keys and values held in 4 bits -----
+# Microscaled floating point: 32 neighbouring elements of a key or value row share a scale 2^(s - 127), a byte s, and are codes of
+# 4 bits (0, 0.5, 1, 1.5, 2, 3, 4, 6 and their negatives): 4.25 bits an element.  A block's s - 127 is floor(log2(its largest
+# magnitude)) - 2, at least -124; elements go to the nearest value, ties to the even code, beyond 6 to 6.  A block with an infinity or
+# a NaN is held as NaN.  A cache unit is uint8 [pages, kv_heads, kv4_head_bytes(head_dim)], 16-byte aligned, pages of 64 tokens; where a
+# page's bytes lie is said in csrc/kv4.h.  Pages, slots and positions that a table or a step names outside of what there is are left
+# alone: nothing is stored for such a token, and attention goes without such a page.
+KV4_PAGE = 64
+
+
+def kv4_head_bytes(hd: int) -> int:
+    """Bytes that a page's 64 tokens of one kv head take: keys and values, codes and scales."""
+    if hd % 32 or not 32 <= hd <= 256:
+        raise KernelError(f"4-bit keys and values: head_dim {hd} must be a multiple of 32, at most 256")
+    return 68 * hd
+
+
+def _kv4_cache(name: str, cache: torch.Tensor, block_table: torch.Tensor, nkv: int, hd: int, page: int) -> None:
+    _dev(name, cache, block_table)
+    _req(page == KV4_PAGE, f"{name}: pages of {KV4_PAGE} tokens")
+    _req(nkv > 0 and cache.dtype == torch.uint8 and cache.dim() == 3 and cache.shape[1:] == (nkv, kv4_head_bytes(hd))
+         and cache.data_ptr() % 16 == 0, f"{name}: cache unit must be uint8 [pages, nkv, {kv4_head_bytes(hd)}], 16-byte aligned")
+    _req(block_table.dim() == 2 and block_table.dtype == torch.int32, f"{name}: block table int32 [slots, pages]")
+
+
+def _same_device(name: str, *tensors) -> None:
+    """All on the current device: its stream is the one that the kernels are launched on."""
+    here = torch.cuda.current_device()
+    for t in tensors:
+        if t is not None and t.device.index != here:
+            raise KernelError(f"{name}: tensor on {t.device}, the current device is cuda:{here}")
+
+
+def _kv4_rows(name: str, positions, seq_of_token, slots, T: int) -> None:
+    _dev(name, positions, seq_of_token, slots)
+    _req(positions.dtype == seq_of_token.dtype == slots.dtype == torch.int32, f"{name}: positions, seq_of_token and slots must be int32")
+    _req(positions.numel() >= T and seq_of_token.numel() >= T, f"{name}: positions shorter than tokens")
+
+
+def rope_kv4_write(qkv: torch.Tensor, cos: Optional[torch.Tensor], sin: Optional[torch.Tensor], positions: torch.Tensor,
+                   seq_of_token: torch.Tensor, slots: torch.Tensor, block_table: torch.Tensor, cache: Optional[torch.Tensor],
+                   nq: int, nkv: int, hd: int, rotary_dim: int, adjacent: bool, page: int, write_cache: bool) -> None:
+    """`rope_kv_write` for a cache of 4-bit keys and values: rotates the queries of the step's rows [T, (nq + 2 nkv) * hd] in
+    place, and puts rotated keys (rounded to the rows' type first) and values into their pages.  No two tokens of a step may
+    stand at the same place of one slot."""
+    name = "rope_kv4_write"
+    _dev(name, qkv, cos, sin)
+    _req(qkv.dim() == 2 and nq >= 0 and qkv.shape[1] == (nq + 2 * nkv) * hd, f"{name}: qkv width is not (nq + 2 nkv) * head_dim")
+    _req(qkv.data_ptr() % 16 == 0, f"{name}: rows must be 16-byte aligned")
+    T = qkv.shape[0]
+    _kv4_rows(name, positions, seq_of_token, slots, T)
+    kv4_head_bytes(hd)
+    _req((cos is None) == (sin is None), f"{name}: both rotary tables, or none")
+    if cos is not None:
+        _req(0 <= rotary_dim <= hd and rotary_dim % 2 == 0, f"{name}: rotary_dim {rotary_dim} must be even, at most {hd}")
+        _req(cos.dtype == sin.dtype == torch.float32 and min(cos.numel(), sin.numel()) >= T * (rotary_dim // 2)
+             and cos.data_ptr() % 16 == 0 and sin.data_ptr() % 16 == 0, f"{name}: rotary tables must be float32 [T, rotary_dim / 2]")
+    if write_cache:
+        _req(cache is not None, f"{name}: no cache to write to")
+        _kv4_cache(name, cache, block_table, nkv, hd, page)
+    _same_device(name, qkv, cos, sin, positions, seq_of_token, slots, block_table, cache)
+    f = _fn("kv4_cache", "br_rope_kv4_write", [_P, c_int, _P, _P, _P, _P, _P, c_int, _P, c_int, c_int, _P] + [c_int] * 8 + [_P])
+    _check(f(_ptr(qkv), _is_bf16(qkv, name), _ptr(cos), _ptr(sin), _ptr(positions), _ptr(seq_of_token), _ptr(slots), slots.numel(),
+             _ptr(block_table), block_table.shape[0], block_table.shape[1], _ptr(cache), cache.shape[0] if cache is not None else 0, T,
+             nq, nkv, hd, rotary_dim if cos is not None else 0, int(adjacent), int(write_cache), _stream()), name)
+
+
+def kv4_read(k_out: torch.Tensor, v_out: torch.Tensor, positions: torch.Tensor, seq_of_token: torch.Tensor, slots: torch.Tensor,
+             block_table: torch.Tensor, cache: torch.Tensor, nkv: int, hd: int, page: int) -> None:
+    """k_out[t], v_out[t] [T, nkv * hd] = what the cache holds for position positions[t] of sequence seq_of_token[t], exactly
+    (bfloat16 or float32).  Rows of padding sequences (slot -1) are left as they are."""
+    name = "kv4_read"
+    _dev(name, k_out, v_out)
+    _req(k_out.dim() == 2 and k_out.shape == v_out.shape and k_out.shape[1] == nkv * hd and k_out.dtype == v_out.dtype,
+         f"{name}: k_out and v_out must be [T, nkv * hd] of one type")
+    _req(k_out.data_ptr() % 16 == 0 and v_out.data_ptr() % 16 == 0, f"{name}: rows must be 16-byte aligned")
+    T = k_out.shape[0]
+    _kv4_rows(name, positions, seq_of_token, slots, T)
+    _kv4_cache(name, cache, block_table, nkv, hd, page)
+    _same_device(name, k_out, v_out, positions, seq_of_token, slots, block_table, cache)
+    f = _fn("kv4_cache", "br_kv4_read", [_P, _P, c_int, _P, _P, _P, c_int, _P, c_int, c_int, _P] + [c_int] * 4 + [_P])
+    _check(f(_ptr(k_out), _ptr(v_out), _is_bf16(k_out, name), _ptr(positions), _ptr(seq_of_token), _ptr(slots), slots.numel(),
+             _ptr(block_table), block_table.shape[0], block_table.shape[1], _ptr(cache), cache.shape[0], T, nkv, hd, _stream()), name)
+
+
+def attention_kv4_splits(n_seqs: int, max_new: int, nq: int, nkv: int, hd: int, max_ctx: int, window: Optional[int] = None) -> int:
+    """Into how many runs the 4-bit attention kernels cut the pages that a row sees (1: none), by the step's shape: sequences,
+    most new tokens of one, an upper bound of the contexts.  With n > 1 they take scratch part_o of T * nq * n * hd and part_ml of
+    T * nq * n * 2 floats, T the step's tokens."""
+    cus = device_cus()
+    tile = 16 if max_new == 1 else 256
+    groups = max(1, n_seqs * nkv * -(-(max_new * (nq // nkv)) // tile))
+    seen = max_ctx if window is None else min(max_ctx, window + max_new)
+    pages = max(1, -(-seen // KV4_PAGE))
+    n = 1
+    if max_new == 1:
+        while n < 64 and n * 8 <= pages and (n * groups < 4 * cus):
+            n *= 2
+    else:
+        while n < 64 and n * 8 <= pages and n * groups * 2 <= cus:
+            n *= 2
+    return n
+
+
+def _attention_kv4(name, q, out, slots, ctx_lens, block_table, cache, B, T, nq, nkv, hd, page, window, scale, nsplit, part_o, part_ml, more=()):
+    _dev(name, out, slots, ctx_lens, part_o, part_ml, *more)
+    _req(q.is_cuda and q.dtype == torch.bfloat16 and out.dtype == torch.bfloat16, f"{name}: bfloat16 only")
+    _kv4_cache(name, cache, block_table, nkv, hd, page)
+    _req(nq > 0 and nq % nkv == 0 and out.dim() == 2 and out.shape[1] == nq * hd and out.shape[0] >= T, f"{name}: out must be [T, nq * hd]")
+    _req(slots.dtype == ctx_lens.dtype == torch.int32 and min(slots.numel(), ctx_lens.numel()) >= B, f"{name}: slots and ctx_lens int32 [B]")
+    _req(scale > 0, f"{name}: the score scale must be positive, not {scale} (the kernels take the row maximum before scaling)")
+    _req(window is None or window > 0, f"{name}: the window must be positive or None, not {window}")
+    _req(1 <= nsplit <= 64, f"{name}: 1 to 64 runs, not {nsplit}")
+    if nsplit > 1:
+        _req(part_o is not None and part_ml is not None and part_o.dtype == part_ml.dtype == torch.float32
+             and part_o.numel() >= T * nq * nsplit * hd and part_ml.numel() >= T * nq * nsplit * 2 and part_o.data_ptr() % 16 == 0,
+             f"{name}: scratch for the runs is too small")
+    _same_device(name, q, out, slots, ctx_lens, block_table, cache, part_o, part_ml, *more)
+
+
+def _q_rows(name: str, q: torch.Tensor, q_stride: int, T: int, width: int) -> None:
+    """`q`'s storage holds T rows of `width` elements, `q_stride` apart, from its first element on."""
+    _req(q_stride >= width and q_stride % 8 == 0 and q.data_ptr() % 16 == 0, f"{name}: query rows must be 16-byte aligned")
+    room = q.untyped_storage().nbytes() // q.element_size() - q.storage_offset()
+    _req(T == 0 or (T - 1) * q_stride + width <= room, f"{name}: q holds fewer than {T} rows of {width}, {q_stride} apart")
+
+
+def attention_decode_kv4(q: torch.Tensor, q_stride: int, out: torch.Tensor, slots: torch.Tensor, ctx_lens: torch.Tensor,
+                         block_table: torch.Tensor, cache: torch.Tensor, B: int, nq: int, nkv: int, hd: int, page: int,
+                         window: Optional[int], scale: float, nsplit: int, part_o: Optional[torch.Tensor] = None,
+                         part_ml: Optional[torch.Tensor] = None) -> None:
+    """`attention_decode_bf16` over a cache of 4-bit keys and values: one new token per sequence, which the cache holds
+    already (`rope_kv4_write`).  Rows of padding sequences, and of sequences of no tokens, are zero.  `nsplit`:
+    `attention_kv4_splits`.  Two calls that may run at the same time need scratch of their own."""
+    name = "attention_decode_kv4"
+    _attention_kv4(name, q, out, slots, ctx_lens, block_table, cache, B, B, nq, nkv, hd, page, window, scale, nsplit, part_o, part_ml)
+    _q_rows(name, q, q_stride, B, nq * hd)
+    f = _fn("attention_kv4", "br_attn_decode_kv4",
+            [_P, c_size_t, _P, _P, _P, _P, c_int, c_int, _P] + [c_int] * 6 + [c_float, c_int, _P, _P, _P])
+    _check(f(_ptr(q), q_stride, _ptr(out), _ptr(slots), _ptr(ctx_lens), _ptr(block_table), block_table.shape[0], block_table.shape[1],
+             _ptr(cache), cache.shape[0], B, nq, nkv, hd, int(window or 0), float(scale), nsplit, _ptr(part_o), _ptr(part_ml), _stream()),
+           name)
+
+
+def attention_prefill_kv4(q: torch.Tensor, q_stride: int, out: torch.Tensor, cu_seqlens: torch.Tensor, slots: torch.Tensor,
+                          ctx_lens: torch.Tensor, block_table: torch.Tensor, cache: torch.Tensor, B: int, max_new: int, nq: int,
+                          nkv: int, hd: int, page: int, window: Optional[int], scale: float, nsplit: int,
+                          part_o: Optional[torch.Tensor] = None, part_ml: Optional[torch.Tensor] = None) -> None:
+    """`attention_prefill_bf16` over a cache of 4-bit keys and values, which holds the new tokens already (`rope_kv4_write`):
+    sequence b's are rows cu_seqlens[b] .. cu_seqlens[b + 1] of `out` and `q`, the last of its ctx_lens[b] tokens; `max_new` is
+    the most of one sequence.  Rows of padding sequences are zero, rows behind the last sequence stay as they are."""
+    name = "attention_prefill_kv4"
+    T = out.shape[0]
+    _attention_kv4(name, q, out, slots, ctx_lens, block_table, cache, B, T, nq, nkv, hd, page, window, scale, nsplit, part_o, part_ml,
+                   (cu_seqlens,))
+    _q_rows(name, q, q_stride, T, nq * hd)
+    _req(cu_seqlens.dtype == torch.int32 and cu_seqlens.numel() >= B + 1, f"{name}: cu_seqlens int32 [B + 1]")
+    _req(0 <= max_new <= T, f"{name}: max_new {max_new} of {T} rows")
+    f = _fn("attention_kv4", "br_attn_prefill_kv4",
+            [_P, c_size_t, _P, _P, _P, _P, _P, c_int, c_int, _P] + [c_int] * 8 + [c_float, c_int, _P, _P, _P])
+    _check(f(_ptr(q), q_stride, _ptr(out), _ptr(cu_seqlens), _ptr(slots), _ptr(ctx_lens), _ptr(block_table), block_table.shape[0],
+             block_table.shape[1], _ptr(cache), cache.shape[0], B, max_new, T, nq, nkv, hd, int(window or 0), float(scale), nsplit,
+             _ptr(part_o), _ptr(part_ml), _stream()), name)
+
+
 # -------------------------------------------------------------------- sampling -----
 def argmax(logits: torch.Tensor, out: torch.Tensor) -> None:
     _dev("argmax", logits, out)
