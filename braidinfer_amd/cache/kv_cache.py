@@ -13,7 +13,8 @@ may differ and the second may be zero (a mixer that keeps one row per token).  W
 inside a head's block is the mixer's business: the attention part of this library keeps
 keys as `[token, head_dim]` after rotation and values transposed as `[head_dim, token]`
 (the operand layout of the matrix-core attention kernels).  A windowed group returns pages
-that lie wholly before the window to its pool after every step.
+that lie wholly before the window to its pool after every step.  A unit whose need says that its
+rows are `held` in 4 bits is storage `[n_pages, kv_heads, bytes of a head's part]` instead (uint8).
 """
 from __future__ import annotations
 
@@ -50,6 +51,9 @@ class CacheNeed:
     # The first `keep_first` positions of a sequence stay readable whatever `window` or `live_from` say (a window that
     # also keeps the sequence's first tokens): the pages that hold them are never returned.
     keep_first: int = 0
+    # In which form the rows lie in the pages: None: elements of the cache's own type; "mxfp4": 4-bit floats with a scale
+    # for every 32 neighbours (4.25 bits an element, `kernels.rope_kv4_write`), keys and values of one width in steps of 32.
+    held: Optional[str] = None
 
     @property
     def key_dim(self) -> int:
@@ -129,27 +133,44 @@ class CacheGroup:
                 (need.tokens_per_row > 1 and (need.window is not None or need.live_from is not None or need.keep_first)):
             raise CacheError(f"a cache unit keeps one row for every tokens_per_row >= 1 tokens, and all of them when "
                              f"that is more than one, got {need}")
+        head_bytes = self._held_bytes(need, page_tokens) if need.held is not None else 0
         self.key_elems = need.kv_heads * page_tokens * need.key_dim        # of one page
         self.page_elems = self.key_elems + need.kv_heads * page_tokens * need.val_dim
         self.storage: Dict[int, torch.Tensor] = {}
         if dtype is not None:
             for u in self.unit_ids:
-                self.storage[u] = torch.zeros((n_pages, self.page_elems), dtype=dtype, device=self.device)
+                shape, kind = ((n_pages, self.page_elems), dtype) if need.held is None else ((n_pages, need.kv_heads, head_bytes), torch.uint8)
+                self.storage[u] = torch.zeros(shape, dtype=kind, device=self.device)
+
+    @staticmethod
+    def _held_bytes(need: CacheNeed, page_tokens: int) -> int:
+        """Bytes of one head's part of a page whose rows are held in another form than the cache's own type."""
+        from ..kernels import KV4_PAGE, kv4_head_bytes
+        if need.held != "mxfp4" or page_tokens != KV4_PAGE or need.val_dim != need.key_dim or need.tokens_per_row != 1 \
+                or need.key_dim % 32 or need.key_dim > 256:
+            raise CacheError(f"a unit held in 4 bits ('mxfp4') keeps keys and values of one width, a multiple of 32 up to 256, a row a "
+                             f"token, in pages of {KV4_PAGE}; got {need} in pages of {page_tokens}")
+        return kv4_head_bytes(need.key_dim)
 
     # -- views of a unit's storage ----------------------------------------------------------
-    def keys(self, unit: int) -> torch.Tensor:
-        """[pages, kv_heads, page_tokens * key_dim]: every head's block of keys, page by page."""
+    def keys(self, unit: int) -> Optional[torch.Tensor]:
+        """[pages, kv_heads, page_tokens * key_dim]: every head's block of keys, page by page; None of rows held in 4 bits."""
+        if self.need.held is not None:
+            return None
         return self.storage[unit][:, :self.key_elems].view(-1, self.need.kv_heads, self.page_tokens * self.need.key_dim)
 
-    def values(self, unit: int) -> torch.Tensor:
-        """[pages, kv_heads, page_tokens * value_dim]."""
+    def values(self, unit: int) -> Optional[torch.Tensor]:
+        """[pages, kv_heads, page_tokens * value_dim]; None of rows held in 4 bits."""
+        if self.need.held is not None:
+            return None
         return self.storage[unit][:, self.key_elems:].view(-1, self.need.kv_heads, self.page_tokens * self.need.val_dim)
 
     def storage_view(self, unit: int) -> torch.Tensor:
         """Keys and values of equal width as one tensor [pages, 2, kv_heads, page_tokens, head_dim]
-        (what this library's attention kernels take); the flat [pages, page elements] otherwise."""
+        (what this library's attention kernels take); the flat [pages, page elements] otherwise; the bytes
+        [pages, kv_heads, bytes of a head's part] of rows held in 4 bits."""
         n = self.need
-        if n.val_dim == n.key_dim:
+        if n.val_dim == n.key_dim and n.held is None:
             return self.storage[unit].view(-1, 2, n.kv_heads, self.page_tokens, n.key_dim)
         return self.storage[unit]
 

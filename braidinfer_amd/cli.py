@@ -14,7 +14,7 @@ Output: the generated text on standard output (token ids when the folder has no
 tokenizer), statistics on standard error, including the reference's `PPTG` line.
 
 Flags beyond the reference: --prompt-ids, --batch-file, --temperature, --top-k, --top-p,
---min-p, --repetition-penalty, --seed, --dtype, --random-weights SEED --preset NAME
+--min-p, --repetition-penalty, --seed, --dtype, --kv-cache, --random-weights SEED --preset NAME
 (--save-folder DIR, --shard-bytes N), --list-weights.
 """
 from __future__ import annotations
@@ -65,6 +65,8 @@ def main(argv: Optional[List[str]] = None) -> int:
     ap.add_argument("--seed", type=int, default=None)
     ap.add_argument("--dtype", choices=["bfloat16", "float32", "bf16", "fp32"], default="bfloat16",
                     help="bfloat16 (bf16) or float32 (fp32)")
+    ap.add_argument("--kv-cache", choices=["mxfp4"], default=None,
+                    help="mxfp4: keys and values in 4 bits (default: in --dtype)")
     ap.add_argument("--random-weights", type=int, metavar="SEED", default=None,
                     help="make a model folder of random weights for --preset instead of reading MODEL")
     ap.add_argument("--preset", default="tiny-a")
@@ -139,7 +141,8 @@ def main(argv: Optional[List[str]] = None) -> int:
         cap_seq = min(max_seq_len, 1 << 20) if max_seq_len else max(longest, 64)
         room = sum(-(-min(len(p) + max_tokens, cap_seq) // 64) * 64 for p in prompts)
         t0 = time.perf_counter()
-        engine = B.Engine.from_folder(model_dir, dtype=args.dtype, max_tokens=max(room, 64), max_seq_len=cap_seq)
+        engine = B.Engine.from_folder(model_dir, dtype=args.dtype, max_tokens=max(room, 64), max_seq_len=cap_seq,
+                                      kv_cache=args.kv_cache)
         print(f"LOAD PROFILE: Engine.from_folder = {(time.perf_counter() - t0) * 1e3:.0f} ms", file=sys.stderr)
         if engine.load_profile is not None:
             print(engine.load_profile.line(), file=sys.stderr)

@@ -1,4 +1,4 @@
-from .spec import PartSpec, LayerSpec, ScheduleEntry, ModelSpec, default_schedule, prenorm_layer
+from .spec import PartSpec, LayerSpec, ScheduleEntry, ModelSpec, default_schedule, prenorm_layer, with_kv_cache
 from .registry import (Architecture, register_architecture, unregister_architecture,
                        registered_architectures, architecture_of, architecture_of_config,
                        read_config_json, config_from_dict, config_from_folder, spec_of, generation_stop_tokens)
@@ -38,7 +38,7 @@ def any_preset(name: str, **overrides):
     raise ConfigError(f"unknown preset {name!r}; known: {sorted(n for p, _ in PRESET_FAMILIES.values() for n in p)}")
 
 __all__ = [
-    "PartSpec", "LayerSpec", "ScheduleEntry", "ModelSpec", "default_schedule", "prenorm_layer",
+    "PartSpec", "LayerSpec", "ScheduleEntry", "ModelSpec", "default_schedule", "prenorm_layer", "with_kv_cache",
     "Architecture", "register_architecture", "unregister_architecture", "registered_architectures",
     "architecture_of", "architecture_of_config", "read_config_json", "config_from_dict",
     "config_from_folder", "spec_of", "generation_stop_tokens", "MistralConfig", "PRESETS", "preset",

@@ -13,8 +13,10 @@ is not.
 """
 from __future__ import annotations
 
-from dataclasses import dataclass, field
+from dataclasses import dataclass, field, replace
 from typing import Any, Dict, List, Optional
+
+from ..errors import ConfigError
 
 
 @dataclass(frozen=True)
@@ -135,6 +137,20 @@ class ModelSpec:
     streams: Optional[int] = None
     # tensors a checkpoint may carry that no part reads (a norm in front of a feed-forward the layer does not have)
     optional_tensors: List[str] = field(default_factory=list)
+
+
+def with_kv_cache(spec: ModelSpec, held: Optional[str]) -> ModelSpec:
+    """`spec` with the keys and values of its attention held in another form (`CacheNeed.held`); None: as it is.  For models whose
+    mixers are all `gqa_attention`, which reads such a cache."""
+    if held is None:
+        return spec
+    if held != "mxfp4":
+        raise ConfigError(f"kv_cache {held!r} is not known; use 'mxfp4' (4-bit floats, 32 to a scale) or None (the model's own type)")
+    kinds = {m.kind for ls in spec.layers for m in [ls.mixer, *ls.more_mixers.values()] if m is not None}
+    if kinds - {"gqa_attention"}:
+        raise ConfigError(f"kv_cache {held!r} is built for models whose mixers are gqa_attention; {spec.architecture} has {sorted(kinds)}")
+    layers = [ls if ls.mixer is None else replace(ls, mixer=PartSpec(ls.mixer.kind, {**ls.mixer.params, "kv_cache": held})) for ls in spec.layers]
+    return replace(spec, layers=layers)
 
 
 def default_schedule(n_layers: int) -> List[ScheduleEntry]:

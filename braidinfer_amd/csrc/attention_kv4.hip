@@ -217,7 +217,7 @@ __global__ __launch_bounds__(256) void attn_decode_kv4_kernel(const bf16* __rest
     if (ctx > seqs.table_pages * KV4_PAGE) ctx = seqs.table_pages * KV4_PAGE;
     const int lo = window > 0 && ctx - window > 0 ? ctx - window : 0;           // the query stands at ctx - 1
     const int pg_lo = lo / KV4_PAGE, npg = ctx > 0 ? (ctx - 1) / KV4_PAGE - pg_lo + 1 : 0;
-    const int pps = (npg + nsplit - 1) / nsplit;
+    const int even = (npg + nsplit - 1) / nsplit, pps = even < 4 ? 4 : even;    // a page for every wave at least
     const int pg_begin = pg_lo + split * pps;
     const int pg_end = pg_begin + pps < pg_lo + npg ? pg_begin + pps : pg_lo + npg;
     if (nsplit > 1 && pg_begin >= pg_end) {             // nothing to add: the join uses no sums of such a run

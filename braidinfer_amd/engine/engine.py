@@ -17,7 +17,7 @@ import torch
 
 from .. import kernels as K
 from ..cache import SequenceCache
-from ..config import config_from_folder, generation_stop_tokens, spec_of
+from ..config import config_from_folder, generation_stop_tokens, spec_of, with_kv_cache
 from ..errors import BraidError, CacheError, ConfigError, KernelError, StepError
 from ..parts import Runtime
 from ..weights import FolderTensors, RandomTensors, write_model_folder
@@ -79,13 +79,14 @@ class Engine:
 
     # ---- construction ------------------------------------------------------------------
     @classmethod
-    def _from_source(cls, config, make_source, dtype, device, max_tokens, max_seq_len, n_slots, use_graphs) -> "Engine":
+    def _from_source(cls, config, make_source, dtype, device, max_tokens, max_seq_len, n_slots, use_graphs,
+                     kv_cache: Optional[str] = None) -> "Engine":
         """Build the model of `config`, size one arena for what its parts keep, and let the
         parts pull their tensors from the source `make_source(specs, allowed, device, dtype)` makes."""
         from ..weights import WeightArena
         device = torch.device(device)
         _require_gpu(device)
-        model = DecoderModel(spec_of(config))
+        model = DecoderModel(with_kv_cache(spec_of(config), kv_cache))
         rt = Runtime(device=device, dtype=parse_dtype(dtype))
         source = make_source(model.weight_specs(), model.optional_names(), device, rt.dtype)
         rt.arena = WeightArena(device, source.resident_bytes())
@@ -98,26 +99,28 @@ class Engine:
     @classmethod
     def from_folder(cls, folder: str, dtype="bfloat16", device="cuda:0", max_tokens: int = 8192,
                     max_seq_len: Optional[int] = None, n_slots: Optional[int] = None,
-                    use_graphs: bool = True) -> "Engine":
+                    use_graphs: bool = True, kv_cache: Optional[str] = None) -> "Engine":
         """A model folder (config.json and model.safetensors, or shards with their index).
+        `kv_cache` "mxfp4" holds keys and values in 4 bits (bfloat16 models whose mixers are GQA attention with
+        heads in steps of 32): a quarter of the memory and of the bytes that attention reads; None: in `dtype`.
         `engine.load_profile.line()` says how the load went (the reference prints a
         `LOAD PROFILE` line, bin/generate.rs:62-68)."""
         config = config_from_folder(folder)
         more_stops = generation_stop_tokens(folder)
         eng = cls._from_source(config, lambda specs, allowed, dev, dt: FolderTensors(folder, specs, dev, dt, allowed),
-                               dtype, device, max_tokens, max_seq_len, n_slots, use_graphs)
+                               dtype, device, max_tokens, max_seq_len, n_slots, use_graphs, kv_cache)
         eng.stop_token_ids += [t for t in more_stops if t not in eng.stop_token_ids]
         return eng
 
     @classmethod
     def random(cls, config, seed: int = 0, dtype="bfloat16", device="cuda:0", max_tokens: int = 8192,
                max_seq_len: Optional[int] = None, n_slots: Optional[int] = None, std: float = 0.02,
-               use_graphs: bool = True, vector_jitter: float = 0.0) -> "Engine":
+               use_graphs: bool = True, vector_jitter: float = 0.0, kv_cache: Optional[str] = None) -> "Engine":
         """Seeded random weights made on the device (no folder): the same bits a
         random-weights folder of that configuration, seed and std holds (bfloat16 N(0, std)
-        matrices, norm weights 1), widened for the 32-bit path."""
+        matrices, norm weights 1), widened for the 32-bit path.  `kv_cache` as in `from_folder`."""
         return cls._from_source(config, lambda specs, allowed, dev, dt: RandomTensors(specs, seed, dev, dt, std, vector_jitter),
-                                dtype, device, max_tokens, max_seq_len, n_slots, use_graphs)
+                                dtype, device, max_tokens, max_seq_len, n_slots, use_graphs, kv_cache)
 
     @staticmethod
     def write_random_folder(folder: str, config, seed: int = 0, std: float = 0.02,
@@ -138,6 +141,23 @@ class Engine:
 
     def length(self, slot: int) -> int:
         return self.cache.length(slot)
+
+    def cache_rows(self, slot: int, unit: int = 0):
+        """(first, keys, values): what the 4-bit cache unit holds of `slot`'s sequence, in the model's type
+        [tokens, kv_heads, head_dim] from position `first` on (a windowed unit has given back what lies before it)."""
+        length = self.cache.length(slot)
+        if unit not in self.cache.group_of_unit or self.cache.unit_group(unit).need.held != "mxfp4":
+            raise CacheError(f"cache unit {unit!r} does not hold rows in 4 bits")
+        g = self.cache.unit_group(unit)
+        first = g.first_page[slot] * g.page_tokens
+        n, nkv, hd = length - first, g.need.kv_heads, g.need.head_dim
+        pos = torch.arange(first, length, dtype=torch.int32, device=self.device)
+        keys, values = (torch.empty((n, nkv * hd), dtype=self.rt.dtype, device=self.device) for _ in range(2))
+        g.sync()
+        if n:
+            K.kv4_read(keys, values, pos, torch.zeros_like(pos), torch.tensor([slot], dtype=torch.int32, device=self.device),
+                       g.table_dev, g.storage[unit], nkv, hd, g.page_tokens)
+        return first, keys.view(n, nkv, hd), values.view(n, nkv, hd)
 
     # ---- the step function -------------------------------------------------------------
     def step(self, entries: Sequence[StepEntry], probe=None) -> torch.Tensor:

@@ -8,6 +8,10 @@ kernels/megakernel_ops.hip:2150-2343: kv head = q head / (nq / nkv) :2192, scale
 rsqrt(head_dim) :2194, causality by loop bound); x += W_o o (compile_attention.rs:333-376).
 A window W limits a query at position i to keys i-W < j <= i (absent in the reference,
 config.rs:416).
+
+With `kv_cache` "mxfp4" the pages hold keys and values in 4 bits, 32 neighbours to a scale (`kernels.rope_kv4_write`), 3.8 times
+as many tokens in the same memory: a key is rotated, rounded to bfloat16 and then held, so a prompt's own tokens are read back
+as the tokens behind them will read them, however a prompt is cut into steps.
 """
 from __future__ import annotations
 
@@ -64,7 +68,8 @@ class GQAAttention(Mixer):
     through_linear_only = True
 
     def __init__(self, hidden_size: int, num_heads: int, num_kv_heads: int, head_dim: int,
-                 window: Optional[int] = None, position: Optional[str] = "rope", scale: Optional[float] = None):
+                 window: Optional[int] = None, position: Optional[str] = "rope", scale: Optional[float] = None,
+                 kv_cache: Optional[str] = None):
         if num_heads <= 0 or num_kv_heads <= 0 or num_heads % num_kv_heads:
             raise ConfigError(f"attention: {num_heads} heads are not a multiple of {num_kv_heads} kv heads")
         if head_dim <= 0 or head_dim % 2:
@@ -73,6 +78,11 @@ class GQAAttention(Mixer):
             raise ConfigError(f"attention: head_dim {head_dim} is beyond what any attention kernel of this library "
                               f"takes ({MAX_HEAD_DIM})")
         self.H, self.nq, self.nkv, self.hd = int(hidden_size), int(num_heads), int(num_kv_heads), int(head_dim)
+        if kv_cache not in (None, "mxfp4"):
+            raise ConfigError(f"attention: kv_cache {kv_cache!r} is not known (None or 'mxfp4')")
+        if kv_cache is not None and (head_dim % 32 or head_dim > 256):
+            raise ConfigError(f"attention: keys and values in 4 bits need a head_dim in steps of 32 up to 256, not {head_dim}")
+        self.kv_cache = kv_cache
         self.window = None if window is None else int(window)
         self.position = position
         self.scale = float(scale) if scale is not None else 1.0 / math.sqrt(self.hd)
@@ -92,12 +102,14 @@ class GQAAttention(Mixer):
         ]
 
     def load(self, tensors: Dict[str, torch.Tensor], prefix: str, rt: Runtime) -> None:
+        if self.kv_cache is not None and not rt.is_bf16:
+            raise ConfigError(f"attention: keys and values in 4 bits go with bfloat16 models, not {rt.dtype}")
         self.rt = rt
         self.w_qkv = fused_layout([tensors[prefix + n + "_proj.weight"] for n in ("q", "k", "v")], rt)
         self.w_o = stream_layout(tensors[prefix + "o_proj.weight"], rt)
 
     def cache_need(self) -> CacheNeed:
-        return CacheNeed(kv_heads=self.nkv, head_dim=self.hd, window=self.window)
+        return CacheNeed(kv_heads=self.nkv, head_dim=self.hd, window=self.window, held=self.kv_cache)
 
     def check_positions(self, encodings) -> None:
         if self.position is None:
@@ -121,6 +133,12 @@ class GQAAttention(Mixer):
         if (tables is None and self._expects_tables) or (tables is not None and not isinstance(tables, RotaryTables)):
             raise StepError(f"attention: the position encoding {self.position!r} gave {type(tables).__name__}, "
                             "rotary tables were expected")
+        if self.kv_cache is not None:
+            linear(h, self.w_qkv, qkv, step.ws)
+            K.rope_kv4_write(qkv, tables.cos if tables else None, tables.sin if tables else None, step.positions, step.seq_of_token,
+                             step.slots, ctx.block_table, ctx.storage, nq, nkv, hd, tables.rotary_dim if tables else 0,
+                             tables.adjacent if tables else False, ctx.page_tokens, ctx.writes_cache)
+            return self._finish(qkv, x, step, ctx, None, False)
         if self._fused_decode(qkv, tables, step, ctx):
             # the kernel that rotates and writes the cache itself reads only its own heads of the
             # step's rows: where their product is cut into runs it adds the runs too
@@ -156,6 +174,20 @@ class GQAAttention(Mixer):
         sizes beyond 256 or not in steps of 16) the one-wave-per-query kernel."""
         T = step.n_tokens
         nq, nkv, hd = self.nq, self.nkv, self.hd
+        if self.kv_cache is not None:
+            B, new = step.n_seqs, 1 if step.is_decode else step.max_new
+            nsplit = K.attention_kv4_splits(B, new, nq, nkv, hd, step.max_ctx_bound, self.window)
+            part_o = part_ml = None
+            if nsplit > 1:
+                part_o = step.ws.get("attn_part_o", (T * nq * nsplit * hd,), torch.float32)
+                part_ml = step.ws.get("attn_part_ml", (T * nq * nsplit * 2,), torch.float32)
+            where = (step.slots, step.ctx_lens, ctx.block_table, ctx.storage, B)
+            sizes = (nq, nkv, hd, ctx.page_tokens, self.window, self.scale, nsplit, part_o, part_ml)
+            if step.is_decode:
+                K.attention_decode_kv4(qkv, qkv.stride(0), o, *where, *sizes)
+            else:
+                K.attention_prefill_kv4(qkv, qkv.stride(0), o, step.cu_seqlens, *where, new, *sizes)
+            return
         if qkv.dtype == torch.bfloat16 and hd % 16 == 0 and hd <= 256 and ctx.page_tokens == 64 and not self.force_simple:
             B = step.n_seqs
             if step.is_decode:

@@ -76,3 +76,50 @@ def test_sizes_that_the_cache_entry_points_refuse():
     # no tokens: nothing to do
     assert w(0, 1, 0, 0, 0, 0, 0, 1, 0, 1, 1, 0, 1, 0, 1, 1, 64, 0, 0, 1, 0) == 0
     assert r(0, 0, 1, 0, 0, 0, 1, 0, 1, 1, 0, 1, 0, 1, 64, 0) == 0
+
+
+def test_models_that_can_hold_keys_and_values_in_4_bits():
+    import braidinfer_amd as B
+    from braidinfer_amd.config import spec_of, with_kv_cache
+    from braidinfer_amd.engine import DecoderModel
+    from braidinfer_amd.errors import ConfigError
+    spec = spec_of(B.preset("mistral-7b-v0.1", num_hidden_layers=2))
+    assert with_kv_cache(spec, None) is spec
+    needs = DecoderModel(with_kv_cache(spec, "mxfp4")).cache_needs()
+    assert [n.held for n in needs.values()] == ["mxfp4"] * 2 and needs[0].window == 4096
+    assert all(n.held is None for n in DecoderModel(spec).cache_needs().values())
+    with pytest.raises(ConfigError, match="int8"):
+        with_kv_cache(spec, "int8")
+    with pytest.raises(ConfigError, match="gqa_attention"):
+        with_kv_cache(spec_of(B.any_preset("kesitar-tiny")), "mxfp4")
+    with pytest.raises(ConfigError, match="head_dim in steps of 32"):
+        DecoderModel(with_kv_cache(spec_of(B.preset("tiny-a")), "mxfp4"))
+    from braidinfer_amd.parts.attention import GQAAttention
+    from braidinfer_amd.parts import Runtime
+    part = GQAAttention(64, 2, 1, 32, kv_cache="mxfp4")
+    with pytest.raises(ConfigError, match="bfloat16"):
+        part.load({}, "", Runtime(device=torch.device("cpu"), dtype=torch.float32))
+    with pytest.raises(ConfigError):
+        GQAAttention(64, 2, 1, 32, kv_cache="mxfp8")
+
+
+def test_units_held_in_4_bits():
+    from braidinfer_amd.cache import CacheNeed, SequenceCache
+    from braidinfer_amd.errors import CacheError
+    c = SequenceCache({0: CacheNeed(3, 64, held="mxfp4"), 1: CacheNeed(3, 64), 2: CacheNeed(3, 64, held="mxfp4")}, {}, max_tokens=200,
+                      dtype=torch.bfloat16)
+    assert len(c.groups) == 2                                             # another form is another group
+    g = c.unit_group(0)
+    assert g.storage[2].shape == (4, 3, 68 * 64) and g.storage[2].dtype == torch.uint8
+    assert c.unit_storage(0) is g.storage[0] and g.keys(0) is None and g.values(0) is None
+    assert c.unit_storage(1).shape == (4, 2, 3, 64, 64) and c.unit_group(1).keys(1) is not None
+    s = c.alloc_slot()
+    c.reserve([s], [130])
+    c.commit([s], [130])
+    assert [len(x.pages[s]) for x in c.groups] == [3, 3]
+    for bad in (CacheNeed(1, 48, held="mxfp4"), CacheNeed(1, 288, held="mxfp4"), CacheNeed(1, 64, value_dim=32, held="mxfp4"), CacheNeed(1, 64, held="fp8"),
+                CacheNeed(1, 64, tokens_per_row=2, held="mxfp4")):
+        with pytest.raises(CacheError, match="mxfp4"):
+            SequenceCache({0: bad}, {}, max_tokens=64, dtype=torch.bfloat16)
+    with pytest.raises(CacheError, match="pages of 64"):
+        SequenceCache({0: CacheNeed(1, 64, held="mxfp4")}, {}, max_tokens=64, page_tokens=32, dtype=torch.bfloat16)
