@@ -25,6 +25,10 @@ __device__ __forceinline__ bf16x8 kv4_zero8() {
     return z;
 }
 
+// A word that all lanes ask for, through the scalar cache: such a load neither waits for the vector loads in flight nor holds them up.
+// (Nothing that a kernel here reads this way is written while it runs.)
+__device__ __forceinline__ int kv4_uniform(const int* p) { return *(const __attribute__((address_space(4))) int*)p; }
+
 // What one query's row can see and where its sequence's pages are
 struct Kv4Seqs {
     const int* slots;
@@ -34,73 +38,216 @@ struct Kv4Seqs {
 };
 
 // ---------------------------------------------------------------------- decode ------
-// One token per sequence.  grid = (runs, nkv * blocks of 16 heads, sequences), block = 256: the 4 waves take the pages of a
-// run in turn, each with keys and values straight from memory into registers, the next page's in flight while one is
-// multiplied, and are joined in LDS in wave order.  Nothing is shared between waves, so nothing passes through LDS before.
-// MP: head size / 32 rounded up to a power of two, the lanes' share of a row (8 MP channels); blocks beyond M are zero.
-template <int M>
-struct Kv4Page {
-    static constexpr int MP = M > 4 ? 8 : M == 3 ? 4 : M;
-    static constexpr int KS = MP == 8 ? 2 : 1, VSETS = MP == 8 ? 2 : 1;
-    unsigned k[4][MP];           // codes of the lane's token in each of the four 16-row tiles
-    unsigned ks[KS];             // their scales, a byte a tile
-    unsigned v[2][VSETS][8];     // codes of 8 tokens x 8 channels in each half of the page
-    u32x2 vs[2][VSETS];          // the 8 tokens' scales
+// One token per sequence.  All pages that a step's tokens see, sequence by sequence for one kv head (and block of GB query heads), then for the
+// next, are one list, of which every workgroup takes as many places in a row: with runs by the longest sequence, or as many for each, those of a
+// batch of unequal lengths differ several times in length, and a workgroup's start (its lengths, table, first page: one wait for the
+// memory each) is paid again for every run.  The lists' lengths are on the device only, so each workgroup adds them up for itself.
+// A sequence and group take KV4_SWITCH places more than their pages, in front of them: what it costs to begin with another one
+// (queries, maxima, joining the waves), in pages.
+#define KV4_SWITCH 4
+struct Kv4Runs {
+    int B, window, groups, wgs, nsplit;          // groups: kv heads x blocks of query heads; nsplit: pieces that a sequence may come in
+    float per_wg, per_piece;                     // a little more than groups / wgs and 1 / (nsplit - 1)
 
-    __device__ __forceinline__ void load(const unsigned char* __restrict__ part, int c, int g) {
-        typedef kv4_layout<M> L;
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const int t = 32 * (j >> 1) + 8 * (c >> 2) + 4 * (j & 1) + (c & 3);
-            const unsigned char* row = part + L::KC + t * (16 * M) + g * (4 * MP);
-            if constexpr (MP == 1) k[j][0] = *(const unsigned*)row;
-            else if constexpr (MP == 2) { const u32x2 w = *(const u32x2*)row; k[j][0] = w[0]; k[j][1] = w[1]; }
-            else {
-#pragma unroll
-                for (int i = 0; i < MP / 4; ++i) {
-                    u32x4 w = {0u, 0u, 0u, 0u};
-                    if (M == MP || (MP / 4) * g + i < M) w = *(const u32x4*)(row + 16 * i);
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) k[j][4 * i + e] = w[e];
-                }
-            }
-        }
-#pragma unroll
-        for (int i = 0; i < KS; ++i) {
-            const int blk = MP == 8 ? 2 * g + i : MP == 4 ? g : MP == 2 ? g >> 1 : 0;
-            ks[i] = 0x7f7f7f7fu;
-            if (M == MP || blk < M) ks[i] = *(const unsigned*)(part + L::KS + (c * M + blk) * 4);
-        }
-#pragma unroll
-        for (int h = 0; h < 2; ++h)
-#pragma unroll
-            for (int s = 0; s < VSETS; ++s) {
-                const int cg = MP == 8 ? 16 * s + c : MP == 4 ? c : MP == 2 ? c & 7 : c & 3, tg = 4 * h + g;
-                u32x4 a = {0u, 0u, 0u, 0u}, b = a;
-                vs[h][s] = u32x2{0x7f7f7f7fu, 0x7f7f7f7fu};
-                if (M == MP || cg < 4 * M) {
-                    const unsigned char* at = part + L::VC + (tg * (4 * M) + cg) * 32;
-                    a = *(const u32x4*)at;
-                    b = *(const u32x4*)(at + 16);
-                    vs[h][s] = *(const u32x2*)(part + L::VS + (tg * M + (cg >> 2)) * 8);
-                }
-#pragma unroll
-                for (int e = 0; e < 4; ++e) { v[h][s][e] = a[e]; v[h][s][4 + e] = b[e]; }
-            }
+    // sequence b's context, the first token that it sees, and the pages between
+    __device__ __forceinline__ int pages(const Kv4Seqs& s, int slot, int length, int& ctx, int& lo) const {
+        ctx = length;
+        if ((unsigned)slot >= (unsigned)s.n_slots || ctx < 0) ctx = 0;
+        if (ctx > s.table_pages * KV4_PAGE) ctx = s.table_pages * KV4_PAGE;
+        lo = window > 0 && ctx - window > 0 ? ctx - window : 0;                // the query stands at ctx - 1
+        return ctx > 0 ? (ctx - 1) / KV4_PAGE - lo / KV4_PAGE + 1 : 0;
+    }
+    // inclusive sums and maxima over the lanes
+    static __device__ __forceinline__ int scan(int x) {
+        x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xf, 0xf, true);       // from the lane 1, 2, 4, 8 below in a row of 16
+        x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xf, 0xf, true);
+        x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xf, 0xf, true);
+        x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xf, 0xf, true);
+        x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xa, 0xf, false);      // a row's last lane to the next row, rows 1 and 3
+        x += __builtin_amdgcn_update_dpp(0, x, 0x143, 0xc, 0xf, false);      // lane 31 to rows 2 and 3
+        return x;
+    }
+    static __device__ __forceinline__ int most(int x) {                      // of numbers that are not negative; in lane 63
+        auto up = [](int a, int b) { return a > b ? a : b; };
+        x = up(x, __builtin_amdgcn_update_dpp(0, x, 0x111, 0xf, 0xf, true));
+        x = up(x, __builtin_amdgcn_update_dpp(0, x, 0x112, 0xf, 0xf, true));
+        x = up(x, __builtin_amdgcn_update_dpp(0, x, 0x114, 0xf, 0xf, true));
+        x = up(x, __builtin_amdgcn_update_dpp(0, x, 0x118, 0xf, 0xf, true));
+        x = up(x, __builtin_amdgcn_update_dpp(0, x, 0x142, 0xa, 0xf, false));
+        return up(x, __builtin_amdgcn_update_dpp(0, x, 0x143, 0xc, 0xf, false));
     }
 };
 
+// The list, as a wave sees it: lane i holds sequence base + i.
+struct Kv4List {
+    int slot, length;               // of the lane's sequence
+    int n, upto, base;              // its places in a group's part of the list, and of all up to it
+    int total, p;                   // places of a group's part; places that a workgroup takes
+
+    static __device__ __forceinline__ int places(const Kv4Runs& r, const Kv4Seqs& s, int slot, int length) {
+        int ctx, lo;
+        const int n = r.pages(s, slot, length, ctx, lo);
+        return n ? n + KV4_SWITCH : 0;
+    }
+    __device__ __forceinline__ void at(const Kv4Runs& r, const Kv4Seqs& s, int from, int sum, int lane) {
+        base = from;
+        slot = from + lane < r.B ? s.slots[from + lane] : -1;
+        length = from + lane < r.B ? s.ctx_lens[from + lane] : 0;
+        n = places(r, s, slot, length);
+        upto = sum + Kv4Runs::scan(n);
+    }
+    __device__ __forceinline__ int end() const { return __builtin_amdgcn_readlane(upto, 63); }
+    __device__ __forceinline__ void start(const Kv4Runs& r, const Kv4Seqs& s, int lane) {
+        at(r, s, 0, 0, lane);
+        int longest = n, sum = n;
+        total = end();
+        if (r.B > WAVE) {
+            for (int b = WAVE + lane; b < r.B; b += WAVE) {
+                const int x = places(r, s, s.slots[b], s.ctx_lens[b]);
+                longest = longest > x ? longest : x;
+                sum += x;
+            }
+            total = __builtin_amdgcn_readlane(Kv4Runs::scan(sum), 63);
+        }
+        longest = __builtin_amdgcn_readlane(Kv4Runs::most(longest), 63);
+        // an even share, a page for each wave at least, and no sequence in more than nsplit pieces (it may begin and end inside a
+        // workgroup's places); the factors are rounded up, so a product that is cut off is the share or more once 1 is added
+        p = 4 + KV4_SWITCH;
+        const int even = (int)((float)total * r.per_wg) + 1, least = (int)((float)longest * r.per_piece) + 1;
+        p = p > even ? p : even;
+        p = p > least ? p : least;
+    }
+    // the sequence that holds place y of a group's part, its places and the place where they begin; y does not fall but to 0
+    __device__ __forceinline__ int find(const Kv4Runs& r, const Kv4Seqs& s, int y, int& own, int& first, int& its_slot, int& its_length, int lane) {
+        if (y < __builtin_amdgcn_readlane(upto, 0) - __builtin_amdgcn_readlane(n, 0)) at(r, s, 0, 0, lane);
+        while (y >= end()) at(r, s, base + WAVE, end(), lane);
+        const int i = __builtin_ctzll(__ballot(upto > y));
+        own = __builtin_amdgcn_readlane(n, i);
+        first = __builtin_amdgcn_readlane(upto, i) - own;
+        its_slot = __builtin_amdgcn_readlane(slot, i);
+        its_length = __builtin_amdgcn_readlane(length, i);
+        return base + i;
+    }
+};
+
+// Place C behind lane offset `off` of a part: a uniform base, 32 bits of offset a lane and what an instruction holds of the rest.
+template <int C> __device__ __forceinline__ const unsigned char* kv4_at(const unsigned char* part, unsigned off) {
+    if constexpr (C < 4064) return part + off + C;
+    else return part + (off + (unsigned)C);
+}
+// Where a lane's share of a page begins: row c, quarter g (see kv4.h)
 template <int M>
+struct Kv4Lane {
+    int c, g;
+    unsigned k, ks, v, vs;
+    __device__ __forceinline__ Kv4Lane(int lane) : c(lane & 15), g(lane >> 4) {
+        typedef kv4_layout<M> L;
+        constexpr int MP = M > 4 ? 8 : M == 3 ? 4 : M;
+        const int blk = MP == 8 ? 2 * g : MP == 4 ? g : MP == 2 ? g >> 1 : 0, cg = MP >= 4 ? c : MP == 2 ? c & 7 : c & 3;
+        k = (8 * (c >> 2) + (c & 3)) * (16 * M) + g * (4 * MP) + L::KC;
+        ks = (c * M + blk) * 4 + L::KS;
+        v = (g * (4 * M) + cg) * 32 + L::VC;
+        vs = (g * M + (cg >> 2)) * 8 + L::VS;
+        asm volatile("" : "+v"(k), "+v"(ks), "+v"(v), "+v"(vs));           // kept, not worked out again for every load
+    }
+};
+
+// MP: head size / 32 rounded up to a power of two, the lanes' share of a row (8 MP channels); blocks beyond M are zero.
+template <int M>
+struct Kv4Keys {
+    static constexpr int MP = M > 4 ? 8 : M == 3 ? 4 : M, KS = MP == 8 ? 2 : 1;
+    unsigned k[4][MP];           // codes of the lane's token in each of the page's four 16-row tiles
+    unsigned ks[KS];             // their scales, a byte a tile
+
+    __device__ __forceinline__ void load(const unsigned char* __restrict__ part, const Kv4Lane<M>& lane) {
+        typedef kv4_layout<M> L;
+        load<0>(part, lane);
+        load<1>(part, lane);
+        load<2>(part, lane);
+        load<3>(part, lane);
+#pragma unroll
+        for (int i = 0; i < KS; ++i) {
+            ks[i] = 0x7f7f7f7fu;
+            if (M == MP || KS * lane.g + i < M) ks[i] = __builtin_nontemporal_load((const unsigned*)(part + lane.ks + 4 * i));
+        }
+    }
+    template <int J> __device__ __forceinline__ void load(const unsigned char* __restrict__ part, const Kv4Lane<M>& lane) {
+        const unsigned char* row = kv4_at<(32 * (J >> 1) + 4 * (J & 1)) * (16 * M)>(part, lane.k);
+        if constexpr (MP == 1) k[J][0] = __builtin_nontemporal_load((const unsigned*)row);
+        else if constexpr (MP == 2) { const u32x2 w = __builtin_nontemporal_load((const u32x2*)row); k[J][0] = w[0]; k[J][1] = w[1]; }
+        else {
+#pragma unroll
+            for (int i = 0; i < MP / 4; ++i) {
+                u32x4 w = {0u, 0u, 0u, 0u};
+                if (M == MP || (MP / 4) * lane.g + i < M) w = __builtin_nontemporal_load((const u32x4*)(row + 16 * i));
+#pragma unroll
+                for (int e = 0; e < 4; ++e) k[J][4 * i + e] = w[e];
+            }
+        }
+    }
+};
+template <int M>
+struct Kv4Values {
+    static constexpr int MP = Kv4Keys<M>::MP, SETS = MP == 8 ? 2 : 1;
+    unsigned v[SETS][8];         // codes of 8 tokens x 8 channels of half a page
+    u32x2 vs[SETS];              // the 8 tokens' scales
+
+    template <int H> __device__ __forceinline__ void load(const unsigned char* __restrict__ part, const Kv4Lane<M>& lane) {
+        set<H, 0>(part, lane);
+        if constexpr (SETS == 2) set<H, 1>(part, lane);
+    }
+    template <int H, int S> __device__ __forceinline__ void set(const unsigned char* __restrict__ part, const Kv4Lane<M>& lane) {
+        u32x4 a = {0u, 0u, 0u, 0u}, b = a;
+        vs[S] = u32x2{0x7f7f7f7fu, 0x7f7f7f7fu};
+        if (M == MP || 16 * S + lane.c < 4 * M) {
+            const unsigned char* at = kv4_at<H * (512 * M) + S * 512>(part, lane.v);
+            a = __builtin_nontemporal_load((const u32x4*)at);
+            b = __builtin_nontemporal_load((const u32x4*)(at + 16));
+            vs[S] = __builtin_nontemporal_load((const u32x2*)(kv4_at<H * (32 * M) + S * 32>(part, lane.vs)));
+        }
+#pragma unroll
+        for (int e = 0; e < 4; ++e) { v[S][e] = a[e]; v[S][4 + e] = b[e]; }
+    }
+};
+
+// GB heads are the columns of the products.  With 4 or 8 of them the 16 columns hold them NK = 4 or 2 times over, and a lane works on
+// the scores of its copy's own tiles only, 16 / GB of the page's tokens each.  Two of the copies then split the values' channels: a
+// converted byte of codes is two channels of one token, and as two neighbouring k-slots of A it meets (p, 0) in the even copy's
+// columns, which gives the one channel, and (0, p) in the odd one's, which gives the other.  So nothing is moved from pairs of channels to
+// pairs of tokens, there are half as many accumulators, and a quarter (half) of the exponentials of a product whose
+// columns are copies or empty: 270 vector instructions a page and wave for 4 heads of 128 instead of 420.
+template <int M, int GB>
 struct Kv4State {
-    static constexpr int MP = Kv4Page<M>::MP;
-    static constexpr int TILES = 2 * MP;        // 16-row tiles of O^T, a channel of the lane's row each
+    static constexpr int MP = Kv4Keys<M>::MP, NK = 16 / GB, OWN = 4 / NK;
+    static constexpr bool SPLIT = GB < 16;
+    static constexpr int TILES = SPLIT ? MP : 2 * MP;
     bf16x8 q[MP];
     f32x4 o[TILES];
     float m, l;
+    bf16x8 pr[2];                  // weights of a page: GB 16, by halves
+    unsigned pw[OWN][2];           // GB 4, 8: of the lane's own tiles, two tokens a word
 
-    // tokens [lo, hi) of the page are seen; `edge`: not all 64
-    __device__ __forceinline__ void page(const Kv4Page<M>& p, int lo, int hi, bool edge, float scale2, int c, int g) {
-        f32x4 s[4];
+    __device__ __forceinline__ void clear() {
+#pragma unroll
+        for (int i = 0; i < TILES; ++i) o[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+        m = -INFINITY;
+        l = 0.f;
+    }
+    // the largest of (or the sum over) the lanes of a head
+    static __device__ __forceinline__ float largest(float x) {
+        if constexpr (GB == 4) x = fmaxf(x, __shfl_xor(x, 4, WAVE));
+        if constexpr (GB <= 8) x = fmaxf(x, __shfl_xor(x, 8, WAVE));
+        x = fmaxf(x, __shfl_xor(x, 16, WAVE));
+        return fmaxf(x, __shfl_xor(x, 32, WAVE));
+    }
+    static __device__ __forceinline__ float sum(float x) {
+        if constexpr (GB == 4) x += __shfl_xor(x, 4, WAVE);
+        if constexpr (GB <= 8) x += __shfl_xor(x, 8, WAVE);
+        x += __shfl_xor(x, 16, WAVE);
+        return x + __shfl_xor(x, 32, WAVE);
+    }
+    // s[j][r]: token 32 (j / 2) + 8 g + 4 (j % 2) + r, head = this lane's column
+    __device__ __forceinline__ void scores(const Kv4Keys<M>& p, f32x4* s) const {
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
             s[j] = f32x4{0.f, 0.f, 0.f, 0.f};
@@ -109,206 +256,395 @@ struct Kv4State {
                 s[j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kv4_to_bf16(p.k[j][w], kv4_scale((p.ks[MP == 8 ? w >> 2 : 0] >> (8 * j)) & 255u)), q[w],
                                                                s[j], 0, 0, 0);
         }
-        // s[j][r]: token 32 (j / 2) + 8 g + 4 (j % 2) + r, head = this lane's column
+    }
+    // tokens [lo, hi) of the page are seen; `edge`: not all 64
+    __device__ __forceinline__ void weights(const f32x4* s, int lo, int hi, bool edge, float scale2, int c, int g) {
+        const int k = c / GB;
+        f32x4 t[OWN];
+#pragma unroll
+        for (int i = 0; i < OWN; ++i)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                if constexpr (GB == 4) t[i][r] = k < 2 ? (k == 0 ? s[0][r] : s[1][r]) : (k == 2 ? s[2][r] : s[3][r]);
+                else if constexpr (GB == 8) t[i][r] = k == 0 ? s[2 * i][r] : s[2 * i + 1][r];
+                else t[i][r] = s[i][r];
+            }
         if (edge) {
 #pragma unroll
-            for (int j = 0; j < 4; ++j)
+            for (int i = 0; i < OWN; ++i) {
+                const int j = GB == 4 ? k : GB == 8 ? 2 * i + k : i, first = 32 * (j >> 1) + 8 * g + 4 * (j & 1);
+                const int a = lo - first, e = hi - first;
 #pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    const int t = 32 * (j >> 1) + 8 * g + 4 * (j & 1) + r;
-                    s[j][r] = t >= lo && t < hi ? s[j][r] : -INFINITY;
-                }
+                for (int r = 0; r < 4; ++r) t[i][r] = r >= a && r < e ? t[i][r] : -INFINITY;
+            }
         }
-        float mx = fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[0][2], s[0][3]));
+        float mx = fmaxf(fmaxf(t[0][0], t[0][1]), fmaxf(t[0][2], t[0][3]));
 #pragma unroll
-        for (int j = 1; j < 4; ++j) mx = fmaxf(mx, fmaxf(fmaxf(s[j][0], s[j][1]), fmaxf(s[j][2], s[j][3])));
-        mx = fmaxf(mx, __shfl_xor(mx, 16, WAVE));
-        mx = fmaxf(mx, __shfl_xor(mx, 32, WAVE)) * scale2;           // the scale is positive
-        const float m_new = fmaxf(m, mx);
-        const float m_use = m_new == -INFINITY ? 0.f : m_new;
-        if (__any(m_new > m)) {
-            const float corr = kv4_exp2(m - m_use);
+        for (int i = 1; i < OWN; ++i) mx = fmaxf(mx, fmaxf(fmaxf(t[i][0], t[i][1]), fmaxf(t[i][2], t[i][3])));
+        mx *= scale2;                                                // the scale is positive
+        // The maximum that is subtracted need not be the largest score: weights up to 2^8 lose nothing in float or bfloat16.  So the
+        // lanes' maxima are brought together, and the sums rescaled, only when one is beyond that.
+        if (__any(mx > m + 8.f)) {
+            const float m_new = fmaxf(m, largest(mx));
+            const float corr = m_new == -INFINITY ? 1.f : kv4_exp2(m - m_new);
+            m = m_new;
             l *= corr;
 #pragma unroll
             for (int i = 0; i < TILES; ++i) o[i] *= corr;
         }
-        m = m_new;
-        float sum = 0.f;
-        bf16x8 pr[2];
+        const float m_use = m == -INFINITY ? 0.f : m;
 #pragma unroll
-        for (int h = 0; h < 2; ++h)
+        for (int i = 0; i < OWN; ++i) {
+            float x[4];
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                x[r] = kv4_exp2(fmaf(t[i][r], scale2, -m_use));
+                l += x[r];
+            }
+            if constexpr (SPLIT) {
+                pw[i][0] = __builtin_bit_cast(unsigned, bf16x2{(bf16)x[0], (bf16)x[1]});
+                pw[i][1] = __builtin_bit_cast(unsigned, bf16x2{(bf16)x[2], (bf16)x[3]});
+            } else {
+#pragma unroll
+                for (int r = 0; r < 4; ++r) pr[i >> 1][4 * (i & 1) + r] = (bf16)x[r];
+            }
+        }
+    }
+    // SPLIT: B of tile J, (p, 0) in the first copy's columns and (0, p) in the second's; sel: `perm`'s selectors that say so
+    template <int J>
+    __device__ __forceinline__ bf16x8 operand(unsigned sel0, unsigned sel1) const {
+        u32x4 b;
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+            unsigned u = pw[GB == 8 ? J >> 1 : 0][x], v = u;
+            // from the copy that worked on tile J: lanes of a row of 16 take the value 4, 8 or 12 lanes on (0x100 +) or back (0x110 +)
+            if constexpr (GB == 8) {
+                if constexpr (J & 1) v = __builtin_amdgcn_update_dpp(u, u, 0x108, 0xf, 0x3, false);
+                else v = __builtin_amdgcn_update_dpp(u, u, 0x118, 0xf, 0xc, false);
+            } else {
+                if constexpr (J == 0) v = __builtin_amdgcn_update_dpp(u, u, 0x114, 0xf, 0x2, false);
+                else if constexpr (J == 1) v = __builtin_amdgcn_update_dpp(u, u, 0x104, 0xf, 0x1, false);
+                else if constexpr (J == 2) v = __builtin_amdgcn_update_dpp(__builtin_amdgcn_update_dpp(u, u, 0x108, 0xf, 0x1, false), u, 0x104, 0xf, 0x2, false);
+                else v = __builtin_amdgcn_update_dpp(__builtin_amdgcn_update_dpp(u, u, 0x10c, 0xf, 0x1, false), u, 0x108, 0xf, 0x2, false);
+            }
+            b[2 * x] = __builtin_amdgcn_perm(0u, v, sel0);
+            b[2 * x + 1] = __builtin_amdgcn_perm(0u, v, sel1);
+        }
+        return __builtin_bit_cast(bf16x8, b);
+    }
+    // two channels of the lane's row, byte B of its tokens' words
+    template <int B>
+    __device__ __forceinline__ void bytes(const unsigned* v, const float* sc, int st, int h, const bf16x8& b0, const bf16x8& b1) {
+        if constexpr (SPLIT) {
+            u32x4 a0, a1;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                a0[e] = __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(v[e], sc[e], B));
+                a1[e] = __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(v[4 + e], sc[4 + e], B));
+            }
+            f32x4& x = o[st * 4 + B];
+            x = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a0), b0, x, 0, 0, 0);
+            x = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a1), b1, x, 0, 0, 0);
+        } else {
+            u32x4 a, b;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                unsigned x, y;
+                kv4_pair<B>(v[2 * e], sc[2 * e], v[2 * e + 1], sc[2 * e + 1], x, y);
+                a[e] = x;
+                b[e] = y;
+            }
+            f32x4 &x = o[st * 8 + 2 * B], &y = o[st * 8 + 2 * B + 1];
+            x = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), pr[h], x, 0, 0, 0);
+            y = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, b), pr[h], y, 0, 0, 0);
+        }
+    }
+    // half H of the page's values
+    template <int H>
+    __device__ __forceinline__ void add(const Kv4Values<M>& p, int lo, int hi, bool edge, unsigned sel0, unsigned sel1, int c, int g) {
+        bf16x8 b0, b1;
+        if constexpr (SPLIT) {
+            b0 = operand<2 * H>(sel0, sel1);
+            b1 = operand<2 * H + 1>(sel0, sel1);
+        }
+#pragma unroll
+        for (int st = 0; st < Kv4Values<M>::SETS; ++st) {
+            unsigned v[8];
+            float sc[8];
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
-                const float x = kv4_exp2(fmaf(s[2 * h + (e >> 2)][e & 3], scale2, -m_use));
-                sum += x;
-                pr[h][e] = (bf16)x;
+                v[e] = p.v[st][e];
+                sc[e] = kv4_scale((p.vs[st][e >> 2] >> (8 * (e & 3))) & 255u);
             }
-        l += sum;
-#pragma unroll
-        for (int h = 0; h < 2; ++h)
-#pragma unroll
-            for (int st = 0; st < Kv4Page<M>::VSETS; ++st) {
-                unsigned v[8];
-                float sc[8];
+            if (edge) {
+                const int a = lo - 32 * H - 8 * g, b = hi - 32 * H - 8 * g;
 #pragma unroll
                 for (int e = 0; e < 8; ++e) {
-                    v[e] = p.v[h][st][e];
-                    sc[e] = kv4_scale((p.vs[h][st][e >> 2] >> (8 * (e & 3))) & 255u);
+                    const bool ok = e >= a && e < b;
+                    v[e] = ok ? v[e] : 0u;
+                    sc[e] = ok ? sc[e] : 1.f;
                 }
-                if (edge) {
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) {
-                        const int t = 32 * h + 8 * g + e;
-                        const bool ok = t >= lo && t < hi;
-                        v[e] = ok ? v[e] : 0u;
-                        sc[e] = ok ? sc[e] : 1.f;
-                    }
-                }
-                if constexpr (MP == 2) {
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) v[e] >>= 16 * (c >> 3);
-                }
-                if constexpr (MP == 1) {
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) v[e] >>= 8 * (c >> 2);
-                }
-                constexpr int PAIRS = MP >= 4 ? 4 : MP;
-                u32x4 a[2 * PAIRS];
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    unsigned x, y;
-                    kv4_pair<0>(v[2 * e], sc[2 * e], v[2 * e + 1], sc[2 * e + 1], x, y);
-                    a[0][e] = x; a[1][e] = y;
-                    if constexpr (PAIRS >= 2) { kv4_pair<1>(v[2 * e], sc[2 * e], v[2 * e + 1], sc[2 * e + 1], x, y); a[2][e] = x; a[3][e] = y; }
-                    if constexpr (PAIRS >= 4) {
-                        kv4_pair<2>(v[2 * e], sc[2 * e], v[2 * e + 1], sc[2 * e + 1], x, y); a[4][e] = x; a[5][e] = y;
-                        kv4_pair<3>(v[2 * e], sc[2 * e], v[2 * e + 1], sc[2 * e + 1], x, y); a[6][e] = x; a[7][e] = y;
-                    }
-                }
-#pragma unroll
-                for (int i = 0; i < 2 * PAIRS; ++i)
-                    o[st * 8 + i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a[i]), pr[h], o[st * 8 + i], 0, 0, 0);
             }
+            if constexpr (MP == 2) {
+#pragma unroll
+                for (int e = 0; e < 8; ++e) v[e] >>= 16 * (c >> 3);
+            }
+            if constexpr (MP == 1) {
+#pragma unroll
+                for (int e = 0; e < 8; ++e) v[e] >>= 8 * (c >> 2);
+            }
+            bytes<0>(v, sc, st, H, b0, b1);
+            if constexpr (MP >= 2) bytes<1>(v, sc, st, H, b0, b1);
+            if constexpr (MP >= 4) {
+                bytes<2>(v, sc, st, H, b0, b1);
+                bytes<3>(v, sc, st, H, b0, b1);
+            }
+        }
     }
-    // the channel of o[tile]'s row r (0..15)
+    // the channel of o[tile]'s row r (0..15); SPLIT: the even copy's, the odd one's is the next
     static __device__ __forceinline__ int channel(int tile, int r) {
-        if constexpr (MP >= 4) return 8 * (r + 16 * (tile >> 3)) + (tile & 7);
-        else if constexpr (MP == 2) return 8 * (r & 7) + 4 * (r >> 3) + tile;
-        else return 8 * (r & 3) + 2 * (r >> 2) + tile;
+        constexpr int PER = MP >= 4 ? 8 : MP == 2 ? 4 : 2;              // channels of a row in one set
+        const int i = SPLIT ? 2 * tile : tile, in = i % PER;
+        if constexpr (MP >= 4) return 8 * (r + 16 * (i / PER)) + in;
+        else if constexpr (MP == 2) return 8 * (r & 7) + 4 * (r >> 3) + in;
+        else return 8 * (r & 3) + 2 * (r >> 2) + in;
     }
 };
 
-template <int M>
-__global__ __launch_bounds__(256) void attn_decode_kv4_kernel(const bf16* __restrict__ q, size_t q_stride, bf16* __restrict__ out,
-                                                              Kv4Seqs seqs, const unsigned char* __restrict__ cache, int nq, int nkv,
-                                                              int window, float scale, int nsplit, float* __restrict__ part_o,
-                                                              float* __restrict__ part_ml) {
-    constexpr int HD = 32 * M, MP = Kv4Page<M>::MP, TILES = Kv4State<M>::TILES;
+// block = 256: the 4 waves take the pages of a stretch in turn, each with keys and values straight from memory into registers, and are
+// joined in LDS in wave order where the stretch ends; nothing else is shared between them.  A wave's next page, of this stretch or
+// the next, is asked for piece by piece, each as soon as the registers that held the present page's are free.
+// `runs.nsplit` 1: a workgroup for every sequence and group, grid = (groups, B); else grid = `runs.wgs`.
+template <int M, int GB>
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(M <= 4 && GB < 16 ? 3 : 2, M <= 4 && GB < 16 ? 3 : 2))) void attn_decode_kv4_kernel(
+    const bf16* __restrict__ q, size_t q_stride, bf16* __restrict__ out, Kv4Seqs seqs, Kv4Runs runs, const unsigned char* __restrict__ cache,
+    int nq, int nkv, float scale, float* __restrict__ part_o, float* __restrict__ part_ml) {
+    typedef Kv4State<M, GB> State;
     typedef kv4_layout<M> L;
-    extern __shared__ float lds[];
-    const int G = nq / nkv, nhb = (G + 15) / 16;
-    const int split = blockIdx.x, kvh = blockIdx.y / nhb, hb = blockIdx.y % nhb, b = blockIdx.z;
+    constexpr int HD = 32 * M, MP = State::MP;
+    constexpr int WSTRIDE = GB * HD + 2 * GB;
+    extern __shared__ float lds[];                      // per wave [GB heads][HD] O, then [GB] m, [GB] l
+    const int G = nq / nkv, nhb = (G + GB - 1) / GB;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int c = lane & 15, g = lane >> 4;
-    const int nheads = (G - hb * 16 < 16) ? G - hb * 16 : 16;
-    const int head0 = kvh * G + hb * 16;
-    const int slot = seqs.slots[b];
-    int ctx = (unsigned)slot < (unsigned)seqs.n_slots ? seqs.ctx_lens[b] : 0;
-    if (ctx > seqs.table_pages * KV4_PAGE) ctx = seqs.table_pages * KV4_PAGE;
-    const int lo = window > 0 && ctx - window > 0 ? ctx - window : 0;           // the query stands at ctx - 1
-    const int pg_lo = lo / KV4_PAGE, npg = ctx > 0 ? (ctx - 1) / KV4_PAGE - pg_lo + 1 : 0;
-    const int even = (npg + nsplit - 1) / nsplit, pps = even < 4 ? 4 : even;    // a page for every wave at least
-    const int pg_begin = pg_lo + split * pps;
-    const int pg_end = pg_begin + pps < pg_lo + npg ? pg_begin + pps : pg_lo + npg;
-    if (nsplit > 1 && pg_begin >= pg_end) {             // nothing to add: the join uses no sums of such a run
-        if ((int)threadIdx.x < nheads) {
-            const size_t at = ((size_t)b * nq + head0 + threadIdx.x) * nsplit + split;
-            part_ml[at * 2] = -INFINITY;
-            part_ml[at * 2 + 1] = 0.f;
+    const Kv4Lane<M> at(lane);
+    const int c = at.c, g = at.g;
+    const bool pieces = runs.nsplit > 1;
+    Kv4List list;
+    int x = 0, end = 0;                                 // this workgroup's places of the list
+    if (pieces) {
+        list.start(runs, seqs, lane);
+        x = (int)blockIdx.x * list.p;
+        const int all = list.total * runs.groups;
+        end = x + list.p < all ? x + list.p : all;
+        // sequences of no tokens are in nobody's part
+        for (int from = blockIdx.x * WAVE; from < runs.B; from += gridDim.x * WAVE) {
+            Kv4List some = list;
+            if (from > 0) some.at(runs, seqs, from, 0, lane);
+            for (unsigned long long none = __ballot(some.n == 0 && from + lane < runs.B); none; none &= none - 1) {
+                const size_t row = (size_t)(from + __builtin_ctzll(none)) * nq * HD;
+                for (int i = threadIdx.x; i < nq * HD; i += 256) out[row + i] = (bf16)0.f;
+            }
         }
-        return;
+        if (x >= end) return;
     }
-    Kv4State<M> st;
-    const bool head_ok = c < nheads;
-    const bf16* qrow = q + (size_t)b * q_stride + (size_t)(head0 + (head_ok ? c : 0)) * HD;
+    // a stretch of pages of one sequence and group (none if the places end before its first page)
+    struct Stretch { int b, group, ctx, lo, first, n, places; bool whole; size_t piece; const int* bt; };
+    auto stretch = [&](int place) {
+        Stretch r;
+        int slot, length;
+        if (pieces) {
+            int begin, own;
+            r.group = place / list.total;
+            r.b = list.find(runs, seqs, place - r.group * list.total, own, begin, slot, length, lane);
+            begin += r.group * list.total;
+            const int from = place - begin, upto = own < end - begin ? own : end - begin;        // of its own places
+            r.places = upto - from;
+            r.first = from > KV4_SWITCH ? from - KV4_SWITCH : 0;
+            r.n = upto - KV4_SWITCH - r.first > 0 ? upto - KV4_SWITCH - r.first : 0;
+            r.whole = r.n == own - KV4_SWITCH;
+            // the first piece is the workgroup's that has its first page
+            r.piece = from <= KV4_SWITCH ? 0 : blockIdx.x - (begin + KV4_SWITCH) / list.p;
+            runs.pages(seqs, slot, length, r.ctx, r.lo);
+        } else {
+            r.b = blockIdx.y;
+            r.group = blockIdx.x;
+            r.first = 0;
+            slot = kv4_uniform(seqs.slots + r.b);
+            length = kv4_uniform(seqs.ctx_lens + r.b);
+            r.n = r.places = runs.pages(seqs, slot, length, r.ctx, r.lo);
+            r.whole = true;
+            r.piece = 0;
+        }
+        r.first += r.lo / KV4_PAGE;
+        r.bt = seqs.table + (size_t)(r.n ? slot : 0) * seqs.table_pages;
+        return r;
+    };
+    Stretch now = stretch(x);
+    // the page that this wave has asked for: number `i` of stretch `ahead`, whose places begin at `xa`; none if part is null
+    Stretch ahead = now;
+    int xa = x, ia = wave;
+    const unsigned char* part = nullptr;
+    auto seek = [&]() {
+        for (;;) {
+            if (ia < ahead.n) {
+                const int pg = __builtin_amdgcn_readfirstlane(kv4_uniform(ahead.bt + ahead.first + ia));
+                if ((unsigned)pg < (unsigned)seqs.n_pages) {
+                    part = cache + ((size_t)pg * nkv + __builtin_amdgcn_readfirstlane(ahead.group / nhb)) * L::BYTES;
+                    return;
+                }
+                ia += 4;
+            } else {
+                xa += ahead.places;
+                if (!pieces || xa >= end) { part = nullptr; return; }
+                ahead = stretch(xa);
+                ia = wave;
+            }
+        }
+    };
+    State st;
+    int nheads, head0;
+    auto queries = [&]() {
+        const int hb = now.group % nhb;
+        head0 = now.group / nhb * G + hb * GB;
+        nheads = G - hb * GB < GB ? G - hb * GB : GB;
+        const bool ok = c % GB < nheads;
+        const bf16* row = q + (size_t)now.b * q_stride + (size_t)(head0 + (ok ? c % GB : 0)) * HD;
 #pragma unroll
-    for (int w = 0; w < MP; ++w) {
-        const int d = g * (8 * MP) + 8 * w;
-        st.q[w] = head_ok && d < HD ? *(const bf16x8*)(qrow + d) : kv4_zero8();
+        for (int w = 0; w < MP; ++w) {
+            const int d = g * (8 * MP) + 8 * w;
+            st.q[w] = ok && d < HD ? *(const bf16x8*)(row + d) : kv4_zero8();
+        }
+    };
+    queries();                                          // before the pages: a wait for them is then none for the pages
+    Kv4Keys<M> keys;
+    Kv4Values<M> v0, v1;
+    seek();
+    if (part) {
+        keys.load(part, at);
+        v0.template load<0>(part, at);
+        v1.template load<1>(part, at);
     }
-#pragma unroll
-    for (int i = 0; i < TILES; ++i) st.o[i] = f32x4{0.f, 0.f, 0.f, 0.f};
-    st.m = -INFINITY;
-    st.l = 0.f;
     const float scale2 = scale * LOG2E;
-    const int* bt = seqs.table + (size_t)(slot < 0 ? 0 : slot) * seqs.table_pages;
-    for (int pi = pg_begin + wave; pi < pg_end; pi += 4) {
-        const int pg = bt[pi];
-        if ((unsigned)pg >= (unsigned)seqs.n_pages) continue;
-        Kv4Page<M> p;
-        p.load(cache + ((size_t)pg * nkv + kvh) * L::BYTES, c, g);
-        const int first = pi * KV4_PAGE, a = lo - first > 0 ? lo - first : 0, e = ctx - first < KV4_PAGE ? ctx - first : KV4_PAGE;
-        st.page(p, a, e, a > 0 || e < KV4_PAGE, scale2, c, g);
-    }
-    st.l += __shfl_xor(st.l, 16, WAVE);
-    st.l += __shfl_xor(st.l, 32, WAVE);
-    // LDS: per wave [16 heads][HD] O, then [16] m, [16] l
-    constexpr int WSTRIDE = 16 * HD + 32;
-    float* my = lds + wave * WSTRIDE;
-#pragma unroll
-    for (int i = 0; i < TILES; ++i)
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-            const int d = Kv4State<M>::channel(i, 4 * g + r);
-            if (M == MP || d < HD) my[c * HD + d] = st.o[i][r];
+    const unsigned odd = c / GB & 1, sel0 = odd ? 0x01000c0cu : 0x0c0c0100u, sel1 = odd ? 0x03020c0cu : 0x0c0c0302u;
+    for (;;) {
+        if (pieces && now.n == 0) return;               // the places end here
+        st.clear();
+        while (part && xa == x) {                       // the page that is there is of this stretch
+            const int tok = (now.first + ia) * KV4_PAGE, a = now.lo - tok > 0 ? now.lo - tok : 0, e = now.ctx - tok < KV4_PAGE ? now.ctx - tok : KV4_PAGE;
+            const bool edge = a > 0 || e < KV4_PAGE;
+            f32x4 s[4];
+            st.scores(keys, s);
+            ia += 4;
+            seek();
+            if (part) keys.load(part, at);
+            st.weights(s, a, e, edge, scale2, c, g);
+            st.template add<0>(v0, a, e, edge, sel0, sel1, c, g);
+            if (part) v0.template load<0>(part, at);
+            st.template add<1>(v1, a, e, edge, sel0, sel1, c, g);
+            if (part) v1.template load<1>(part, at);
         }
-    if (g == 0) { my[16 * HD + c] = st.m; my[16 * HD + 16 + c] = st.l; }
-    __syncthreads();
-    for (int e = threadIdx.x; e < nheads * HD; e += 256) {
-        const int h = e / HD, d = e % HD;
-        float mx = -INFINITY;
+        st.l = State::sum(st.l);
+        float* my = lds + wave * WSTRIDE;
+        const int copy = c / GB, h = c % GB;
+        if (copy < (State::SPLIT ? 2 : 1)) {
 #pragma unroll
-        for (int w = 0; w < 4; ++w) mx = fmaxf(mx, lds[w * WSTRIDE + 16 * HD + h]);
-        const float use = mx == -INFINITY ? 0.f : mx;
-        float sum = 0.f, o = 0.f;
+            for (int i = 0; i < State::TILES; ++i)
 #pragma unroll
-        for (int w = 0; w < 4; ++w) {
-            const float f = kv4_exp2(lds[w * WSTRIDE + 16 * HD + h] - use);
-            sum += lds[w * WSTRIDE + 16 * HD + 16 + h] * f;
-            o += lds[w * WSTRIDE + h * HD + d] * f;
+                for (int r = 0; r < 4; ++r) {
+                    const int d = State::channel(i, 4 * g + r) + copy;
+                    if (M == MP || d < HD) my[h * HD + d] = st.o[i][r];
+                }
         }
-        const int head = head0 + h;
-        if (nsplit == 1) out[((size_t)b * nq + head) * HD + d] = (bf16)(sum == 0.f ? 0.f : o / sum);
-        else {
-            const size_t at = ((size_t)b * nq + head) * nsplit + split;
-            part_o[at * HD + d] = o;
-            if (d == 0) { part_ml[at * 2] = mx; part_ml[at * 2 + 1] = sum; }
+        if (g == 0 && copy == 0) { my[GB * HD + h] = st.m; my[GB * HD + GB + h] = st.l; }
+        __syncthreads();
+        for (int i = threadIdx.x; i < nheads * HD; i += 256) {
+            const int hh = i / HD, d = i % HD;
+            float mx = -INFINITY;
+#pragma unroll
+            for (int w = 0; w < 4; ++w) mx = fmaxf(mx, lds[w * WSTRIDE + GB * HD + hh]);
+            const float use = mx == -INFINITY ? 0.f : mx;
+            float sum = 0.f, o = 0.f;
+#pragma unroll
+            for (int w = 0; w < 4; ++w) {
+                const float f = kv4_exp2(lds[w * WSTRIDE + GB * HD + hh] - use);
+                sum += lds[w * WSTRIDE + GB * HD + GB + hh] * f;
+                o += lds[w * WSTRIDE + hh * HD + d] * f;
+            }
+            const size_t row = (size_t)now.b * nq + head0 + hh;
+            if (now.whole) out[row * HD + d] = (bf16)(sum == 0.f ? 0.f : o / sum);
+            else {
+                const size_t i_ = row * runs.nsplit + now.piece;
+                part_o[i_ * HD + d] = o;
+                if (d == 0) { part_ml[i_ * 2] = mx; part_ml[i_ * 2 + 1] = sum; }
+            }
         }
+        x += now.places;
+        if (!pieces || x >= end) return;
+        now = stretch(x);
+        queries();
+        __syncthreads();
     }
 }
 
 // The runs of a row added in their order: out = sum_i 2^(m_i - M) o_i / sum_i 2^(m_i - M) l_i.  A wave a row (token, head).
 // `last` (null: none): the number of tokens that sequences hold; rows behind them have no runs and stay as they are.
+// RUNS: rows of single tokens, in as many pieces each as the list's places say; those of one are there already.
+template <bool RUNS>
 __global__ __launch_bounds__(256) void attn_kv4_join_kernel(const float* __restrict__ part_o, const float* __restrict__ part_ml,
                                                             bf16* __restrict__ out, size_t rows, int nq, int hd, int nsplit,
-                                                            const int* __restrict__ last) {
+                                                            const int* __restrict__ last, Kv4Seqs seqs, Kv4Runs runs, int G, int gb) {
     const size_t row = (size_t)blockIdx.x * 4 + (threadIdx.x >> 6);
     const int lane = threadIdx.x & 63;
     if (row >= rows || (last && row >= (size_t)(*last > 0 ? *last : 0) * nq)) return;
-    // runs are at most 64, one a lane
-    const float m = lane < nsplit ? part_ml[(row * nsplit + lane) * 2] : -INFINITY;
-    const float l = lane < nsplit ? part_ml[(row * nsplit + lane) * 2 + 1] : 0.f;
+    // runs are at most 64, one a lane; 16 lanes take 64 channels, so that a run's row is hd / 64 groups of them and the others take
+    // further runs at the same time.  Everything is asked for before it is known how many runs there are: of the others nothing is used.
+    const float m_ = lane < nsplit ? part_ml[(row * nsplit + lane) * 2] : -INFINITY;
+    const float l_ = lane < nsplit ? part_ml[(row * nsplit + lane) * 2 + 1] : 0.f;
+    const int per = (hd + 63) / 64, sub = (lane >> 4) / per, many = 4 / per, d = ((lane >> 4) % per) * 64 + (lane & 15) * 4;
+    auto fetch = [&](int i) { return i < nsplit && sub < many && d < hd ? *(const f32x4*)(part_o + (row * nsplit + i) * hd + d) : f32x4{0.f, 0.f, 0.f, 0.f}; };
+    f32x4 x[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) x[j] = fetch(j * many + sub);
+    int n_runs = nsplit;
+    if (RUNS) {
+        const int b = __builtin_amdgcn_readfirstlane((int)(row / nq)), head = __builtin_amdgcn_readfirstlane((int)(row % nq));
+        Kv4List list;
+        list.start(runs, seqs, lane);
+        while (b >= list.base + WAVE) list.at(runs, seqs, list.base + WAVE, list.end(), lane);
+        const int own = __builtin_amdgcn_readlane(list.n, b - list.base);
+        const int group = head / G * ((G + gb - 1) / gb) + head % G / gb;
+        const int first = __builtin_amdgcn_readlane(list.upto, b - list.base) - own + group * list.total;
+        n_runs = own ? (first + own - 1) / list.p - (first + KV4_SWITCH) / list.p + 1 : 1;
+        if (n_runs == 1) return;
+    }
+    const float m = lane < n_runs ? m_ : -INFINITY, l = lane < n_runs ? l_ : 0.f;
     const float mx = wave_max(m);
     const float f = l == 0.f ? 0.f : kv4_exp2(m - (mx == -INFINITY ? 0.f : mx));
     const float sum = wave_sum(l * f);
     const float inv = sum == 0.f ? 0.f : 1.f / sum;
-    for (int d = lane * 4; d < hd; d += 256) {
-        f32x4 o = {0.f, 0.f, 0.f, 0.f};
-        for (int i = 0; i < nsplit; ++i) {
-            const float w = __shfl(f, i, WAVE);
-            if (w == 0.f) continue;                           // a run without a token has written no sums
-            o += w * *(const f32x4*)(part_o + (row * nsplit + i) * hd + d);
+    f32x4 o = {0.f, 0.f, 0.f, 0.f};
+    for (int i0 = 0; i0 < n_runs; i0 += 4 * many) {
+        if (i0 > 0) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) x[j] = fetch(i0 + j * many + sub);
         }
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const int i = i0 + j * many + sub;
+            const float w = __shfl(f, i < n_runs ? i : 0, WAVE);
+            if (i < n_runs && w != 0.f) o += w * x[j];         // a run without a token has written no sums
+        }
+    }
+    if (sub >= many) o = f32x4{0.f, 0.f, 0.f, 0.f};
+    if (per <= 2) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[e] += __shfl_xor(o[e], 32, WAVE);
+    }
+    if (per == 1) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[e] += __shfl_xor(o[e], 16, WAVE);
+    }
+    if (sub == 0 && d < hd) {
         bf16x4 r;
 #pragma unroll
         for (int e = 0; e < 4; ++e) r[e] = (bf16)(o[e] * inv);
@@ -584,10 +920,11 @@ __global__ __launch_bounds__(NW * 64) void attn_prefill_kv4_kernel(const bf16* _
 
 #define KV4_SIZES(F) F(1) F(2) F(3) F(4) F(5) F(6) F(7) F(8)
 
+template <bool RUNS>
 static int kv4_join(const float* part_o, const float* part_ml, void* out, long long tokens, int nq, int hd, int nsplit, const int* last,
-                    hipStream_t s) {
+                    const Kv4Seqs& seqs, const Kv4Runs& runs, int G, int gb, hipStream_t s) {
     const size_t rows = (size_t)tokens * nq;
-    attn_kv4_join_kernel<<<(unsigned)((rows + 3) / 4), 256, 0, s>>>(part_o, part_ml, (bf16*)out, rows, nq, hd, nsplit, last);
+    attn_kv4_join_kernel<RUNS><<<(unsigned)((rows + 3) / 4), 256, 0, s>>>(part_o, part_ml, (bf16*)out, rows, nq, hd, nsplit, last, seqs, runs, G, gb);
     return br_check_launch();
 }
 
@@ -596,19 +933,28 @@ extern "C" int br_attn_decode_kv4(const void* q, size_t q_stride, void* out, con
                                   float scale, int nsplit, float* part_o, float* part_ml, hipStream_t s) {
     if (hd % 32 || hd < 32 || hd > 256 || nkv < 1 || nq < nkv || nq % nkv || B < 0 || B > 65535 || nsplit < 1 || nsplit > 64 ||
         table_pages > 0x7fffffff / KV4_PAGE || (nsplit > 1 && (!part_o || !part_ml))) return BR_BAD_ARG;
-    const int nhb = (nq / nkv + 15) / 16;
-    if ((long long)nkv * nhb > 65535) return BR_BAD_ARG;
+    // heads that share a kv head go as columns of one product: 4, 8 or 16 at a time
+    const int G = nq / nkv, gb = G <= 4 ? 4 : G <= 8 ? 8 : 16, groups = nkv * ((G + gb - 1) / gb);
+    if ((long long)B * nq > 0x7fffffffLL) return BR_BAD_ARG;
+    const int cus = br_device_cus(), all = (cus > 0 ? cus : 256) * 3;      // what is resident of the kernels for heads of up to 128
+    const long long seen = window > 0 && (window + 2LL * KV4_PAGE - 2) / KV4_PAGE < table_pages ? (window + 2LL * KV4_PAGE - 2) / KV4_PAGE : table_pages;
+    const long long pages = B * seen * groups, places = pages + (long long)B * groups * KV4_SWITCH;        // of the list at most
+    if (places > 0x3fffffffLL) return BR_TOO_LARGE;
     if (B == 0) return BR_OK;
-    const dim3 grid(nsplit, nkv * nhb, B);
-    const size_t lds = 4 * (16 * (size_t)hd + 32) * sizeof(float);
+    const int wgs = (int)((pages + 3) / 4 < all ? (pages + 3) / 4 > 0 ? (pages + 3) / 4 : 1 : all);
+    const Kv4Runs runs = {B, window, groups, wgs, nsplit, (float)(1.00001 * groups / wgs), (float)(1.00001 / (nsplit > 1 ? nsplit - 1 : 1))};
+    const dim3 grid = nsplit > 1 ? dim3(wgs) : dim3(groups, B);
+    const size_t lds = 4 * ((size_t)gb * hd + 2 * gb) * sizeof(float);
     const Kv4Seqs seqs = {slots, ctx_lens, table, n_slots, table_pages, n_pages};
-#define CASE(M_) case M_: \
-        if (lds > 65536 && hipFuncSetAttribute((const void*)attn_decode_kv4_kernel<M_>, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds) != hipSuccess) return BR_LAUNCH_FAILED; \
-        attn_decode_kv4_kernel<M_><<<grid, 256, lds, s>>>((const bf16*)q, q_stride, (bf16*)out, seqs, (const unsigned char*)cache, nq, nkv, window, scale, nsplit, part_o, part_ml); break;
+#define GO(M_, GB_) { \
+        if (lds > 65536 && hipFuncSetAttribute((const void*)attn_decode_kv4_kernel<M_, GB_>, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds) != hipSuccess) return BR_LAUNCH_FAILED; \
+        attn_decode_kv4_kernel<M_, GB_><<<grid, 256, lds, s>>>((const bf16*)q, q_stride, (bf16*)out, seqs, runs, (const unsigned char*)cache, nq, nkv, scale, part_o, part_ml); }
+#define CASE(M_) case M_: if (gb == 4) GO(M_, 4) else if (gb == 8) GO(M_, 8) else GO(M_, 16) break;
     switch (hd / 32) { KV4_SIZES(CASE) }
 #undef CASE
+#undef GO
     const int rc = br_check_launch();
-    return rc != BR_OK || nsplit == 1 ? rc : kv4_join(part_o, part_ml, out, B, nq, hd, nsplit, nullptr, s);
+    return rc != BR_OK || nsplit == 1 ? rc : kv4_join<true>(part_o, part_ml, out, B, nq, hd, nsplit, nullptr, seqs, runs, G, gb, s);
 }
 
 extern "C" int br_attn_prefill_kv4(const void* q, size_t q_stride, void* out, const int* cu_seqlens, const int* slots, const int* ctx_lens,
@@ -638,5 +984,5 @@ extern "C" int br_attn_prefill_kv4(const void* q, size_t q_stride, void* out, co
     switch (hd / 32) { KV4_SIZES(CASE) }
 #undef CASE
     const int rc = br_check_launch();
-    return rc != BR_OK || nsplit == 1 ? rc : kv4_join(part_o, part_ml, out, n_tokens, nq, hd, nsplit, cu_seqlens + B, s);
+    return rc != BR_OK || nsplit == 1 ? rc : kv4_join<false>(part_o, part_ml, out, n_tokens, nq, hd, nsplit, cu_seqlens + B, seqs, Kv4Runs{}, 1, 1, s);
 }

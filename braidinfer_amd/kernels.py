@@ -1955,17 +1955,24 @@ def attention_kv4_splits(n_seqs: int, max_new: int, nq: int, nkv: int, hd: int, 
     most new tokens of one, an upper bound of the contexts.  With n > 1 they take scratch part_o of T * nq * n * hd and part_ml of
     T * nq * n * 2 floats, T the step's tokens."""
     cus = device_cus()
-    tile = 16 if max_new == 1 else 256
-    groups = max(1, n_seqs * nkv * -(-(max_new * (nq // nkv)) // tile))
     seen = max_ctx if window is None else min(max_ctx, window + max_new)
-    pages = max(1, -(-seen // KV4_PAGE))
-    n = 1
+    pages = max(1, -(-seen // KV4_PAGE) + (window is not None))
     if max_new == 1:
-        while n < 64 and n * 8 <= pages and (n * groups < 4 * cus):
-            n *= 2
-    else:
-        while n < 64 and n * 8 <= pages and n * groups * 2 <= cus:
-            n *= 2
+        # One workgroup for a sequence and kv head takes 5 us and 0.4 for each page; cut into equal shares of all pages with a second
+        # launch that joins them, 11 us and the time of all bytes (8 kv heads of 128, both ways, us: one sequence of 700 tokens 8.3 / 12.3,
+        # 1,500 11.5 / 10.2; 8 of 128 to 2,048 15.9 / 13.6; 24 of 1,500 13.9 / 17.8; 32 of 128 to 8,192 52 / 38; 64 of 128 to 2,048 19.5 / 27.4,
+        # of 4,160 49 / 61, of 128 to 8,192 63 / 62; 16 of 32,768 194 / 99).  The more of them there are, the longer the one way stays
+        # ahead: the bytes of all then take their time either way.
+        heads = nq // nkv
+        groups = n_seqs * nkv * -(-heads // (4 if heads <= 4 else 8 if heads <= 8 else 16))
+        if pages <= min(80, 16 + groups // 8):
+            return 1
+        # the most pieces of a sequence that the scratch holds: eight times its even share, as one that is longer than the others has
+        return max(2, min(64, -(-pages // 4) + 1, 2 + 24 * cus // max(1, groups)))
+    groups = max(1, n_seqs * nkv * -(-(max_new * (nq // nkv)) // 256))
+    n = 1
+    while n < 64 and n * 8 <= pages and n * groups * 2 <= cus:
+        n *= 2
     return n
 
 
