@@ -3,7 +3,7 @@
 // Per (query row, kv head) the online softmax m' = max(m, s), c = 2^(m - m'), l = l c + p, o = o c + p v with scores in base 2
 // (scaled by scale * log2 e once), in float.  Codes become bfloat16 on their way into the matrix instructions: a code times its
 // scale is exact there, so keys, values and queries enter exactly and only the probabilities are rounded (to bfloat16, half a
-// step of 2^-8 each, which the sum over the keys averages).  The instructions that take 4-bit operands with their scales as they
+// step of 2^-8 each, which the sum over the keys averages; their sum l is taken of the rounded ones).  The instructions that take 4-bit operands with their scales as they
 // are would need the queries as two 8-bit parts, and add their products less exactly: up to 2e-5 of sum |q k| away for normal
 // values, against 1e-7 this way.
 //
@@ -25,9 +25,22 @@ __device__ __forceinline__ bf16x8 kv4_zero8() {
     return z;
 }
 
+// sum + p[0] + p[1] in float.  The weights' sum is taken of the weights as they are rounded for the product with the values: what rounding
+// does to a weight that outweighs the others then goes out again in the division.
+__device__ __forceinline__ float kv4_add_pair(bf16x2 p, float sum) {
+    return __builtin_amdgcn_fdot2_f32_bf16(p, bf16x2{(bf16)1.f, (bf16)1.f}, sum, false);
+}
+
 // A word that all lanes ask for, through the scalar cache: such a load neither waits for the vector loads in flight nor holds them up.
 // (Nothing that a kernel here reads this way is written while it runs.)
 __device__ __forceinline__ int kv4_uniform(const int* p) { return *(const __attribute__((address_space(4))) int*)p; }
+
+// A barrier that orders what lies in LDS and no more: loads from memory stay in flight over it (__syncthreads waits for them).
+__device__ __forceinline__ void kv4_lds_barrier() {
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+}
 
 // What one query's row can see and where its sequence's pages are
 struct Kv4Seqs {
@@ -253,7 +266,7 @@ struct Kv4State {
             s[j] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
             for (int w = 0; w < MP; ++w)
-                s[j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kv4_to_bf16(p.k[j][w], kv4_scale((p.ks[MP == 8 ? w >> 2 : 0] >> (8 * j)) & 255u)), q[w],
+                s[j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kv4_to_bf16(p.k[j][w], kv4_scale_of(p.ks[MP == 8 ? w >> 2 : 0], j)), q[w],
                                                                s[j], 0, 0, 0);
         }
     }
@@ -299,14 +312,15 @@ struct Kv4State {
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
                 x[r] = kv4_exp2(fmaf(t[i][r], scale2, -m_use));
-                l += x[r];
             }
+            const bf16x2 a = {(bf16)x[0], (bf16)x[1]}, b = {(bf16)x[2], (bf16)x[3]};
+            l = kv4_add_pair(b, kv4_add_pair(a, l));
             if constexpr (SPLIT) {
-                pw[i][0] = __builtin_bit_cast(unsigned, bf16x2{(bf16)x[0], (bf16)x[1]});
-                pw[i][1] = __builtin_bit_cast(unsigned, bf16x2{(bf16)x[2], (bf16)x[3]});
+                pw[i][0] = __builtin_bit_cast(unsigned, a);
+                pw[i][1] = __builtin_bit_cast(unsigned, b);
             } else {
-#pragma unroll
-                for (int r = 0; r < 4; ++r) pr[i >> 1][4 * (i & 1) + r] = (bf16)x[r];
+                bf16x8& p = pr[i >> 1];
+                p[4 * (i & 1)] = a[0]; p[4 * (i & 1) + 1] = a[1]; p[4 * (i & 1) + 2] = b[0]; p[4 * (i & 1) + 3] = b[1];
             }
         }
     }
@@ -374,7 +388,7 @@ struct Kv4State {
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
                 v[e] = p.v[st][e];
-                sc[e] = kv4_scale((p.vs[st][e >> 2] >> (8 * (e & 3))) & 255u);
+                sc[e] = kv4_scale_of(p.vs[st][e >> 2], e & 3);
             }
             if (edge) {
                 const int a = lo - 32 * H - 8 * g, b = hi - 32 * H - 8 * g;
@@ -653,32 +667,33 @@ __global__ __launch_bounds__(256) void attn_kv4_join_kernel(const float* __restr
 }
 
 // --------------------------------------------------------------------- prefill ------
-// Several tokens per sequence.  A workgroup takes 32 NW rows of one kv head and sequence, row = token * G + head, 32 a wave, and
+// Several tokens per sequence.  A workgroup takes `tile_rows` <= 32 NW rows of one kv head and sequence, row = token * G + head, 32 a wave, and
 // walks the pages that they see.  A page's codes come to registers while the page before is multiplied, are turned into
 // bfloat16 once for all waves and lie in LDS in the order of the matrix operands, 1 KB a wave-read, two pages deep; one barrier a page.
 // Chunk [half][k-step][lane] of the keys: 8 channels of the key that row lane % 32 of a 32-key block stands for.  Chunk [32 channels]
 // [16 tokens][lane] of the values: 8 tokens of a channel.  (A code and its scale become bfloat16 in half an instruction; read by
 // every wave for itself they would cost NW times as many.)
 //
-// Values that are NaN (scale 255) would spoil rows that do not see them, since 0 * NaN is NaN: a page that holds any is said so, and
-// is multiplied with zeros in their place, NaN going into the accumulators of the rows that see them only.
+// Values that are NaN (scale 255) would spoil rows that do not see them, since 0 * NaN is NaN: they go into LDS as zeros, and which tokens'
+// they were beside them, and NaN goes into the accumulators of the rows that see them only.
 __device__ __forceinline__ int kv4_key_of_row(int c) { return 16 * (c >> 4) + 8 * ((c >> 2) & 1) + 4 * ((c >> 3) & 1) + (c & 3); }
 __device__ __forceinline__ int kv4_row_of_key(int u) { return (u & 3) | (((u >> 2) & 1) << 3) | (((u >> 3) & 1) << 2) | (u & 16); }
 // Place of a channel's row among a value chunk's 32: turned so that the 16 lanes that write different rows at a time reach different banks
 __device__ __forceinline__ int kv4_value_row(int row, int i2) { return row ^ ((row >> 4) | ((i2 & 3) << 1)); }
 
 template <int M, int NW>
-__global__ __launch_bounds__(NW * 64) void attn_prefill_kv4_kernel(const bf16* __restrict__ q, size_t q_stride, bf16* __restrict__ out,
+__global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(NW == 4 && M > 4 ? 1 : 2, 2))) void attn_prefill_kv4_kernel(const bf16* __restrict__ q, size_t q_stride, bf16* __restrict__ out,
                                                                    const int* __restrict__ cu_seqlens, Kv4Seqs seqs,
                                                                    const unsigned char* __restrict__ cache, int nq, int nkv, int window,
-                                                                   float scale, const PrefillOrder order, int n_tokens, int nsplit,
+                                                                   float scale, const PrefillOrder order, int n_tokens, int tile_rows, int nsplit,
                                                                    float* __restrict__ part_o, float* __restrict__ part_ml) {
-    constexpr int HD = 32 * M, NT = NW * 64, ROWS = 32 * NW;
+    constexpr int HD = 32 * M, NT = NW * 64;
     constexpr int KB = KV4_PAGE * HD * 2, STAGE = 2 * KB;                       // bytes of a page's keys; keys and values
-    constexpr int UNITS = 64 * M, UPT = (UNITS + NT - 1) / NT;                  // 32-element units of each; per thread
+    constexpr int UNITS = 64 * M, UPT = (UNITS + NT - 1) / NT;                    // units of 32 elements of the keys, as many of the values; of each a thread
     typedef kv4_layout<M> L;
     extern __shared__ __attribute__((aligned(1024))) unsigned char dsm[];
     int* nan_page = (int*)(dsm + 2 * STAGE);                                    // [2]: the page in a stage that holds NaN values, + 1
+    unsigned char* nan_tokens = dsm + 2 * STAGE + 16;                           // [2][M blocks][8 bytes]: which tokens' values those are
     int kvh, b, tile, split = 0;
     if (nsplit > 1) {                                                           // grid (tiles * runs, nkv, B)
         kvh = blockIdx.y;
@@ -689,11 +704,11 @@ __global__ __launch_bounds__(NW * 64) void attn_prefill_kv4_kernel(const bf16* _
     const int t0 = cu_seqlens[b], n_new = cu_seqlens[b + 1] - t0;
     const int G = nq / nkv;
     const long long rows_total = (long long)n_new * G;
-    if (t0 < 0 || t0 + n_new > n_tokens || (long long)tile * ROWS >= rows_total) return;        // the whole workgroup leaves together
+    if (t0 < 0 || t0 + n_new > n_tokens || (long long)tile * tile_rows >= rows_total) return;        // the whole workgroup leaves together
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int row0 = tile * ROWS + wave * 32;
+    const int row0 = tile * tile_rows + wave * 32;
     const int c = lane & 31, g = lane >> 5;
-    const int last = (int)rows_total - 1;
+    const int last = (int)(rows_total < (long long)(tile + 1) * tile_rows ? rows_total : (long long)(tile + 1) * tile_rows) - 1;       // of the tile's
     const bool wave_ok = row0 <= last, row_ok = row0 + c <= last;
     const int rr = row_ok ? row0 + c : last;
     const int tok = rr / G, head = kvh * G + rr % G;
@@ -702,9 +717,9 @@ __global__ __launch_bounds__(NW * 64) void attn_prefill_kv4_kernel(const bf16* _
     const bool there = (unsigned)slot < (unsigned)seqs.n_slots;
     const int ctx = there ? seqs.ctx_lens[b] : 0, start = ctx - n_new;
     const int pq = start + tok;
-    const int w_last = row0 + 31 < last ? row0 + 31 : last, g_last = tile * ROWS + ROWS - 1 < last ? tile * ROWS + ROWS - 1 : last;
+    const int w_last = row0 + 31 < last ? row0 + 31 : last, g_last = last;
     const int pq_min_w = start + (wave_ok ? row0 : last) / G, pq_max_w = start + w_last / G;
-    const int pq_min_g = start + tile * ROWS / G, pq_max_g = start + g_last / G;
+    const int pq_min_g = start + tile * tile_rows / G, pq_max_g = start + g_last / G;
     int first_pg = window > 0 && pq_min_g - window + 1 > 0 ? (pq_min_g - window + 1) / KV4_PAGE : 0;
     int last_pg = pq_max_g < 0 ? -1 : pq_max_g / KV4_PAGE;
     if (last_pg >= seqs.table_pages) last_pg = seqs.table_pages - 1;
@@ -729,22 +744,25 @@ __global__ __launch_bounds__(NW * 64) void attn_prefill_kv4_kernel(const bf16* _
     const float scale2 = scale * LOG2E;
 
     // A unit of the keys: a block of a token (token unit % 64, block unit / 64); of the values: 8 tokens of 4 channels, half a group of 8.
-    // 16 neighbouring units of the values lie in 16 groups of channels, whose rows reach different banks.
+    // 16 neighbouring units of the values lie in 16 groups of channels, whose rows reach different banks.  For heads of 128 and 8 waves
+    // the first four convert and the others, on the same SIMDs, are at their products meanwhile: units spread over all waves are
+    // slower (8,192 tokens: 647 us against 615; all of them behind the products 715).
     auto value_cg = [](int u) { return M % 4 == 0 ? (u & 15) + 16 * (u >> 8) : u % (4 * M); };
     auto value_half = [](int u) { return M % 4 == 0 ? (u >> 4) & 1 : u / (32 * M); };
     auto value_tg = [](int u) { return M % 4 == 0 ? (u >> 5) & 7 : u / (4 * M) & 7; };
+    // Waves without rows, the last ones, convert where a tile has such; the first ones in full tiles (8,192 tokens: 547 us against 585 by the last).
+    const int unit0 = (tile_rows < 32 * NW ? NW - 1 - wave : wave) * 64 + lane;
     u32x4 kr[UPT], va[UPT], vb[UPT];
     u32x2 vsr[UPT];
     unsigned ksr[UPT];
     auto fetch = [&](const unsigned char* part) {
 #pragma unroll
         for (int i = 0; i < UPT; ++i) {
-            const int u = tid + i * NT;
+            const int u = unit0 + i * NT;
             if (UNITS % NT == 0 || u < UNITS) {
-                const int t = u & 63, blk = u >> 6;
+                const int t = u & 63, blk = u >> 6, cg = value_cg(u), tg = value_tg(u);
                 kr[i] = *(const u32x4*)(part + L::KC + t * (16 * M) + blk * 16);
                 ksr[i] = part[L::KS + kv4_key_scale(t, blk, M)];
-                const int cg = value_cg(u), tg = value_tg(u);
                 const unsigned char* at = part + L::VC + (tg * (4 * M) + cg) * 32;
                 va[i] = *(const u32x4*)at;
                 vb[i] = *(const u32x4*)(at + 16);
@@ -757,29 +775,43 @@ __global__ __launch_bounds__(NW * 64) void attn_prefill_kv4_kernel(const bf16* _
         unsigned char* st = dsm + buf * STAGE;
 #pragma unroll
         for (int i = 0; i < UPT; ++i) {
-            const int u = tid + i * NT;
+            const int u = unit0 + i * NT;
             if (UNITS % NT == 0 || u < UNITS) {
-                const int t = u & 63, blk = u >> 6;
+                const int t = u & 63, blk = u >> 6, krow = kv4_row_of_key(t & 31);
                 const float ks = kv4_scale(ksr[i]);
-                const int krow = kv4_row_of_key(t & 31);
 #pragma unroll
                 for (int w = 0; w < 4; ++w)
                     *(bf16x8*)(st + (((t >> 5) * 2 * M + 2 * blk + (w >> 1)) * 64 + (w & 1) * 32 + krow) * 16) = kv4_to_bf16(kr[i][w], ks);
                 const int cg = value_cg(u), tg = value_tg(u), half = value_half(u);
                 unsigned v[8];
                 float sc[8];
-                bool nan = false;
+                u32x2 vs = vsr[i];
 #pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    const unsigned s8 = (vsr[i][e >> 2] >> (8 * (e & 3))) & 255u;
-                    v[e] = (e < 4 ? va[i][e & 3] : vb[i][e & 3]) >> (16 * half);
-                    sc[e] = kv4_scale(s8);
-                    const bool ok = 8 * tg + e < live;
-                    nan |= ok && s8 == 255u;
-                    v[e] = ok ? v[e] : 0u;
-                    sc[e] = ok ? sc[e] : 1.f;
+                for (int e = 0; e < 8; ++e) v[e] = (e < 4 ? va[i][e & 3] : vb[i][e & 3]) >> (16 * half);
+                if (live < KV4_PAGE) {                                  // what is not written yet: zeros with a scale of 1
+                    const int n = live - 8 * tg;
+#pragma unroll
+                    for (int e = 0; e < 8; ++e)
+                        if (e >= n) {
+                            v[e] = 0u;
+                            vs[e >> 2] = (vs[e >> 2] & ~(255u << (8 * (e & 3)))) | (127u << (8 * (e & 3)));
+                        }
                 }
-                if (nan) nan_page[buf] = pi + 1;
+                // a byte of 255 in either word: all of its lower bits carry into the one above, which is set as well
+                unsigned bad = 0;
+                if (((((vs[0] & 0x7f7f7f7fu) + 0x01010101u) & vs[0]) | (((vs[1] & 0x7f7f7f7fu) + 0x01010101u) & vs[1])) & 0x80808080u) {
+                    nan_page[buf] = pi + 1;
+#pragma unroll
+                    for (int e = 0; e < 8; ++e)
+                        if ((vs[e >> 2] >> (8 * (e & 3)) & 255u) == 255u) {
+                            bad |= 1u << e;
+                            v[e] = 0u;
+                            vs[e >> 2] ^= 128u << (8 * (e & 3));        // 127: 1
+                        }
+                }
+                nan_tokens[(buf * M + (cg >> 2)) * 8 + tg] = (unsigned char)bad;     // the same from all units of the block
+#pragma unroll
+                for (int e = 0; e < 8; ++e) sc[e] = kv4_scale_of(vs[e >> 2], e & 3);
                 u32x4 a[4];
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
@@ -798,36 +830,58 @@ __global__ __launch_bounds__(NW * 64) void attn_prefill_kv4_kernel(const bf16* _
             }
         }
     };
-    // the next page from pi on that is there, or last_pg + 1
+    // The numbers of 64 pages lie in the lanes, so that no turn waits for the table.  `next_page`: the next page from pi on that is there
+    // (its number in `number`), or last_pg + 1.
+    int held = first_pg, numbers = held + lane <= last_pg ? bt[held + lane] : 0, number = 0;
     auto next_page = [&](int pi) {
-        while (pi <= last_pg && (unsigned)bt[pi] >= (unsigned)seqs.n_pages) ++pi;
+        for (; pi <= last_pg; ++pi) {
+            if (pi >= held + 64) {
+                held = pi;
+                numbers = held + lane <= last_pg ? bt[held + lane] : 0;
+            }
+            number = __builtin_amdgcn_readlane(numbers, pi - held);
+            if ((unsigned)number < (unsigned)seqs.n_pages) break;
+        }
         return pi;
     };
+    auto part_of = [&]() { return cache + ((size_t)number * nkv + kvh) * L::BYTES; };
 
     if (tid < 2) nan_page[tid] = 0;
     int pi = next_page(first_pg);
     __syncthreads();
     if (pi <= last_pg) {
-        fetch(cache + ((size_t)bt[pi] * nkv + kvh) * L::BYTES);
+        fetch(part_of());
         put(0, ctx - pi * KV4_PAGE, pi);
     }
-    __syncthreads();
+    int pn = next_page(pi + 1);
+    if (pn <= last_pg) fetch(part_of());
+    kv4_lds_barrier();
     for (int buf = 0; pi <= last_pg; buf ^= 1) {
-        const int pn = next_page(pi + 1);
-        if (pn <= last_pg) fetch(cache + ((size_t)bt[pn] * nkv + kvh) * L::BYTES);
+        const int pm = next_page(pn + 1);
+        auto bring = [&]() {
+            if (pn <= last_pg) put(buf ^ 1, ctx - pn * KV4_PAGE, pn);
+            if (pm <= last_pg) fetch(part_of());
+        };
         const unsigned char* st = dsm + buf * STAGE;
-        const bool has_nan = nan_page[buf] == pi + 1;
+        if (__builtin_amdgcn_readfirstlane(nan_page[buf]) == pi + 1) {
+            // tokens [a, e) of the page are seen by this lane's row
+            const int kb = pi * KV4_PAGE, a = window > 0 && pq - window + 1 - kb > 0 ? pq - window + 1 - kb : 0, e = pq + 1 - kb < KV4_PAGE ? pq + 1 - kb : KV4_PAGE;
+            const unsigned long long seen = row_ok && a < e ? (~0ULL >> (64 - (e - a))) << a : 0;
 #pragma unroll
-        for (int half = 0; half < 2; ++half) {
+            for (int i = 0; i < M; ++i)
+                if (seen & ((const unsigned long long*)nan_tokens)[buf * M + i]) {
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) o[i][r] = NAN;
+                }
+        }
+        auto block = [&](int half) {
             const int kb = pi * KV4_PAGE + 32 * half;
-            // blocks that no row of this wave sees are skipped
-            if (!wave_ok || kb > pq_max_w || (window > 0 && kb + 31 <= pq_min_w - window)) continue;
+            const unsigned char* ks = st + (half * 2 * M * 64 + lane) * 16;
             f32x16 s;
 #pragma unroll
             for (int r = 0; r < 16; ++r) s[r] = 0.f;
 #pragma unroll
-            for (int k = 0; k < 2 * M; ++k)
-                s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(*(const bf16x8*)(st + ((half * 2 * M + k) * 64 + lane) * 16), qf[k], s, 0, 0, 0);
+            for (int k = 0; k < 2 * M; ++k) s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(*(const bf16x8*)(ks + k * 1024), qf[k], s, 0, 0, 0);
             // s[r]: key kb + 16 (r / 8) + 8 g + r % 8, row = this lane's column
             const bool whole = row0 + 31 <= last && kb + 31 <= pq_min_w && (window <= 0 || kb > pq_max_w - window);
             if (!whole) {
@@ -841,62 +895,48 @@ __global__ __launch_bounds__(NW * 64) void attn_prefill_kv4_kernel(const bf16* _
             float mx = fmaxf(fmaxf(s[0], s[1]), s[2]);
 #pragma unroll
             for (int r = 3; r < 15; r += 2) mx = fmaxf(fmaxf(mx, s[r]), s[r + 1]);
-            mx = fmaxf(mx, s[15]);
-            mx = fmaxf(mx, __shfl_xor(mx, 32, WAVE)) * scale2;               // the scale is positive
-            const float m_new = fmaxf(m, mx);
-            const float m_use = m_new == -INFINITY ? 0.f : m_new;
-            if (__any(m_new > m)) {
-                const float corr = kv4_exp2(m - m_use);
+            mx = fmaxf(mx, s[15]) * scale2;                                  // the scale is positive
+            if (__any(mx > m + 8.f)) {                                       // see Kv4State::weights
+                const float m_new = fmaxf(m, fmaxf(mx, __shfl_xor(mx, 32, WAVE)));
+                const float corr = m_new == -INFINITY ? 1.f : kv4_exp2(m - m_new);
+                m = m_new;
                 l *= corr;
 #pragma unroll
                 for (int i = 0; i < M; ++i)
 #pragma unroll
                     for (int r = 0; r < 16; ++r) o[i][r] *= corr;
             }
-            m = m_new;
+            const float m_use = m == -INFINITY ? 0.f : m;
             float sum0 = 0.f, sum1 = 0.f;
             bf16x8 p[2];
 #pragma unroll
             for (int r = 0; r < 16; r += 2) {
                 const float x = kv4_exp2(fmaf(s[r], scale2, -m_use)), y = kv4_exp2(fmaf(s[r + 1], scale2, -m_use));
-                sum0 += x;
-                sum1 += y;
-                p[r >> 3][r & 7] = (bf16)x;
-                p[r >> 3][(r & 7) + 1] = (bf16)y;
+                const bf16x2 w = {(bf16)x, (bf16)y};
+                if (r & 2) sum1 = kv4_add_pair(w, sum1);
+                else sum0 = kv4_add_pair(w, sum0);
+                p[r >> 3][r & 7] = w[0];
+                p[r >> 3][(r & 7) + 1] = w[1];
             }
             l += sum0 + sum1;
+            const unsigned char* vs = st + KB + half * 2048;
 #pragma unroll
             for (int i = 0; i < M; ++i)
 #pragma unroll
-                for (int x = 0; x < 2; ++x) {
-                    bf16x8 v = *(const bf16x8*)(st + KB + ((i * 4 + 2 * half + x) * 64 + 32 * g + kv4_value_row(c, i)) * 16);
-                    if (has_nan) {
-                        unsigned gone = 0;                              // tokens 16 x + 8 g + e of the half whose block i is NaN
-#pragma unroll
-                        for (int e = 0; e < 8; ++e) {
-                            const bool n = (float)v[e] != (float)v[e];
-                            const unsigned long long who = __ballot(n);
-                            if ((unsigned)who) gone |= 1u << e;
-                            if (who >> 32) gone |= 1u << (8 + e);
-                            if (n) v[e] = (bf16)0.f;
-                        }
-                        bool seen = false;
-#pragma unroll
-                        for (int e = 0; e < 16; ++e) {
-                            const int key = kb + 16 * x + e;
-                            seen |= (gone >> e & 1) && row_ok && key <= pq && (window <= 0 || key > pq - window);
-                        }
-                        if (seen) {
-#pragma unroll
-                            for (int r = 0; r < 16; ++r) o[i][r] = NAN;
-                        }
-                    }
-                    o[i] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(v, p[x], o[i], 0, 0, 0);
-                }
-        }
-        if (pn <= last_pg) put(buf ^ 1, ctx - pn * KV4_PAGE, pn);
-        __syncthreads();
+                for (int x = 0; x < 2; ++x)
+                    o[i] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(*(const bf16x8*)(vs + (4 * i + x) * 1024 + (32 * g + kv4_value_row(c, i)) * 16), p[x], o[i],
+                                                                   0, 0, 0);
+        };
+        // halves that no row of this wave sees are left out
+        const int kb = pi * KV4_PAGE;
+        const bool s0 = wave_ok && kb <= pq_max_w && (window <= 0 || kb + 31 > pq_min_w - window);
+        const bool s1 = wave_ok && kb + 32 <= pq_max_w && (window <= 0 || kb + 63 > pq_min_w - window);
+        if (s0) block(0);
+        if (s1) block(1);
+        bring();
+        kv4_lds_barrier();
         pi = pn;
+        pn = pm;
     }
     l += __shfl_xor(l, 32, WAVE);
     if (!row_ok) return;
@@ -961,28 +1001,37 @@ extern "C" int br_attn_prefill_kv4(const void* q, size_t q_stride, void* out, co
                                    const int* table, int n_slots, int table_pages, const void* cache, int n_pages, int B, int max_new,
                                    int n_tokens, int nq, int nkv, int hd, int window, float scale, int nsplit, float* part_o, float* part_ml,
                                    hipStream_t s) {
-    constexpr int NW = 8;
     if (hd % 32 || hd < 32 || hd > 256 || nkv < 1 || nkv > 65535 || nq < nkv || nq % nkv || B < 0 || B > 65535 || max_new < 0 || nsplit < 1 ||
         nsplit > 64 || table_pages > 0x7fffffff / KV4_PAGE || (long long)n_tokens * nq > 0x7fffffffLL || n_tokens < max_new || (nsplit > 1 && (!part_o || !part_ml))) return BR_BAD_ARG;
     const long long rows = (long long)max_new * (nq / nkv);
-    if (rows > 0x7fffffffLL - 32 * NW) return BR_BAD_ARG;
+    if (rows > 0x7fffffffLL - 256) return BR_BAD_ARG;
     if (B == 0 || max_new == 0) return BR_OK;
+    // 8 waves convert a page once for 256 rows.  4 waves, two workgroups to a compute unit, where 8 would leave units without one or
+    // the last tiles alone: a prompt of 67 tokens 9.0 us against 11.3, 512 25.7 / 28.4, 2,048 79 / 82, but 4,096 183 / 167, 8,192 666 / 615.
+    const int cus = br_device_cus() > 0 ? br_device_cus() : 256;
+    const bool wide = hd <= 128 && (nsplit > 1 || (rows + 255) / 256 * nkv * B > cus);      // larger heads have no registers for 8 waves
+    const int most = wide ? 256 : 128;
+    const long long tiles = (rows + most - 1) / most;
     PrefillOrder order = {};
     dim3 grid;
-    // the order counts in tiles of 128 rows: half as many rows in tiles of twice as many
-    if (!prefill_order(order, grid, (rows + 1) / 2, nkv, B, br_device_cus(), hd <= 128 ? 2 : 1)) return BR_BAD_ARG;
+    int tile_rows = most;
     if (nsplit > 1) {
-        const long long x = (rows + 32 * NW - 1) / (32 * NW) * nsplit;
-        if (x > 0x7fffffffLL) return BR_BAD_ARG;
-        grid = dim3((unsigned)x, nkv, B);
-    }
-    const size_t lds = 2 * (size_t)2 * KV4_PAGE * hd * 2 + 16;
+        // tiles of about equal height: 67 tokens of 4 heads are 160 and 108 rows, not 256 and 12
+        tile_rows = (int)(((rows + tiles - 1) / tiles + 31) / 32 * 32);
+        if (tiles * nsplit > 0x7fffffffLL) return BR_BAD_ARG;
+        grid = dim3((unsigned)(tiles * nsplit), nkv, B);
+    } else if (!prefill_order(order, grid, wide ? (rows + 1) / 2 : rows, nkv, B, cus, !wide && hd <= 128 ? 2 : 1)) return BR_BAD_ARG;   // it counts in tiles of 128
+    const size_t lds = 2 * (size_t)2 * KV4_PAGE * hd * 2 + 16 + 2 * (hd / 32) * 8;
     const Kv4Seqs seqs = {slots, ctx_lens, table, n_slots, table_pages, n_pages};
-#define CASE(M_) case M_: \
-        if (hipFuncSetAttribute((const void*)attn_prefill_kv4_kernel<M_, NW>, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds) != hipSuccess) return BR_LAUNCH_FAILED; \
-        attn_prefill_kv4_kernel<M_, NW><<<grid, NW * 64, lds, s>>>((const bf16*)q, q_stride, (bf16*)out, cu_seqlens, seqs, (const unsigned char*)cache, nq, nkv, window, scale, order, n_tokens, nsplit, part_o, part_ml); break;
-    switch (hd / 32) { KV4_SIZES(CASE) }
+#define GO(M_, NW_) { \
+        if (hipFuncSetAttribute((const void*)attn_prefill_kv4_kernel<M_, NW_>, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds) != hipSuccess) return BR_LAUNCH_FAILED; \
+        attn_prefill_kv4_kernel<M_, NW_><<<grid, NW_ * 64, lds, s>>>((const bf16*)q, q_stride, (bf16*)out, cu_seqlens, seqs, (const unsigned char*)cache, nq, nkv, window, scale, order, n_tokens, tile_rows, nsplit, part_o, part_ml); }
+#define CASE(M_) case M_: GO(M_, 4) break;
+#define BOTH(M_) case M_: if (wide) GO(M_, 8) else GO(M_, 4) break;
+    switch (hd / 32) { BOTH(1) BOTH(2) BOTH(3) BOTH(4) CASE(5) CASE(6) CASE(7) CASE(8) }
+#undef BOTH
 #undef CASE
+#undef GO
     const int rc = br_check_launch();
     return rc != BR_OK || nsplit == 1 ? rc : kv4_join<false>(part_o, part_ml, out, n_tokens, nq, hd, nsplit, cu_seqlens + B, seqs, Kv4Runs{}, 1, 1, s);
 }

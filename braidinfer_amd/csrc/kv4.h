@@ -29,8 +29,12 @@ __device__ __forceinline__ int kv4_key_scale(int t, int blk, int m) {       // p
 typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
 typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
 
-// 2^(s - 127) as a float; 255 gives infinity, which the conversions below take as NaN (as they do NaN)
+// 2^(s - 127) as a float; 255 gives infinity, which the conversions below take as NaN (as they do NaN).  They look at the exponent of
+// their scale only: what stands in its sign and fraction does not matter (65,536 words of random bits), so that a byte of a
+// word of scales needs a shift and no mask.
 __device__ __forceinline__ float kv4_scale(unsigned s) { return __uint_as_float(s << 23); }
+
+__device__ __forceinline__ float kv4_scale_of(unsigned word, int byte) { return __uint_as_float(byte < 3 ? word << (23 - 8 * byte) : word >> 1); }
 
 // 8 codes of a word as bfloat16, times `scale`
 __device__ __forceinline__ bf16x8 kv4_to_bf16(unsigned w, float scale) {

@@ -1969,11 +1969,10 @@ def attention_kv4_splits(n_seqs: int, max_new: int, nq: int, nkv: int, hd: int, 
             return 1
         # the most pieces of a sequence that the scratch holds: eight times its even share, as one that is longer than the others has
         return max(2, min(64, -(-pages // 4) + 1, 2 + 24 * cus // max(1, groups)))
-    groups = max(1, n_seqs * nkv * -(-(max_new * (nq // nkv)) // 256))
-    n = 1
-    while n < 64 and n * 8 <= pages and n * groups * 2 <= cus:
-        n *= 2
-    return n
+    # tiles of 256 rows (128 for heads beyond 128) that leave compute units without work: as many runs as fill them once, of 8 pages at
+    # least (67 tokens behind 16,344: 608 us whole, 79 in 8 runs, 50 in 16, 73 in 20; 512 behind none 21 us whole, 28 in 2 runs)
+    groups = max(1, n_seqs * nkv * -(-(max_new * (nq // nkv)) // (256 if hd <= 128 else 128)))
+    return max(1, min(64, cus // groups, pages // 8))
 
 
 def _attention_kv4(name, q, out, slots, ctx_lens, block_table, cache, B, T, nq, nkv, hd, page, window, scale, nsplit, part_o, part_ml, more=()):
