@@ -958,6 +958,16 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(NW == 4
         }
 }
 
+// LDS beyond 64 KB is asked for once for every kernel and device (`told`, a bit a device: a kernel always asks for the same).
+static bool kv4_allow(const void* kernel, size_t lds, unsigned long long& told) {
+    int dev = 0;
+    if (hipGetDevice(&dev) != hipSuccess || dev < 0) return false;
+    if (dev < 64 && (__atomic_load_n(&told, __ATOMIC_RELAXED) >> dev & 1)) return true;
+    if (hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds) != hipSuccess) return false;
+    if (dev < 64) __atomic_fetch_or(&told, 1ULL << dev, __ATOMIC_RELAXED);
+    return true;
+}
+
 #define KV4_SIZES(F) F(1) F(2) F(3) F(4) F(5) F(6) F(7) F(8)
 
 template <bool RUNS>
@@ -987,7 +997,8 @@ extern "C" int br_attn_decode_kv4(const void* q, size_t q_stride, void* out, con
     const size_t lds = 4 * ((size_t)gb * hd + 2 * gb) * sizeof(float);
     const Kv4Seqs seqs = {slots, ctx_lens, table, n_slots, table_pages, n_pages};
 #define GO(M_, GB_) { \
-        if (lds > 65536 && hipFuncSetAttribute((const void*)attn_decode_kv4_kernel<M_, GB_>, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds) != hipSuccess) return BR_LAUNCH_FAILED; \
+        static unsigned long long told; \
+        if (lds > 65536 && !kv4_allow((const void*)attn_decode_kv4_kernel<M_, GB_>, lds, told)) return BR_LAUNCH_FAILED; \
         attn_decode_kv4_kernel<M_, GB_><<<grid, 256, lds, s>>>((const bf16*)q, q_stride, (bf16*)out, seqs, runs, (const unsigned char*)cache, nq, nkv, scale, part_o, part_ml); }
 #define CASE(M_) case M_: if (gb == 4) GO(M_, 4) else if (gb == 8) GO(M_, 8) else GO(M_, 16) break;
     switch (hd / 32) { KV4_SIZES(CASE) }
@@ -1024,7 +1035,8 @@ extern "C" int br_attn_prefill_kv4(const void* q, size_t q_stride, void* out, co
     const size_t lds = 2 * (size_t)2 * KV4_PAGE * hd * 2 + 16 + 2 * (hd / 32) * 8;
     const Kv4Seqs seqs = {slots, ctx_lens, table, n_slots, table_pages, n_pages};
 #define GO(M_, NW_) { \
-        if (hipFuncSetAttribute((const void*)attn_prefill_kv4_kernel<M_, NW_>, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds) != hipSuccess) return BR_LAUNCH_FAILED; \
+        static unsigned long long told; \
+        if (lds > 65536 && !kv4_allow((const void*)attn_prefill_kv4_kernel<M_, NW_>, lds, told)) return BR_LAUNCH_FAILED; \
         attn_prefill_kv4_kernel<M_, NW_><<<grid, NW_ * 64, lds, s>>>((const bf16*)q, q_stride, (bf16*)out, cu_seqlens, seqs, (const unsigned char*)cache, nq, nkv, window, scale, order, n_tokens, tile_rows, nsplit, part_o, part_ml); }
 #define CASE(M_) case M_: GO(M_, 4) break;
 #define BOTH(M_) case M_: if (wide) GO(M_, 8) else GO(M_, 4) break;

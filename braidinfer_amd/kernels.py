@@ -1882,26 +1882,50 @@ def kv4_head_bytes(hd: int) -> int:
     return 68 * hd
 
 
-def _kv4_cache(name: str, cache: torch.Tensor, block_table: torch.Tensor, nkv: int, hd: int, page: int) -> None:
-    _dev(name, cache, block_table)
-    _req(page == KV4_PAGE, f"{name}: pages of {KV4_PAGE} tokens")
-    _req(nkv > 0 and cache.dtype == torch.uint8 and cache.dim() == 3 and cache.shape[1:] == (nkv, kv4_head_bytes(hd))
-         and cache.data_ptr() % 16 == 0, f"{name}: cache unit must be uint8 [pages, nkv, {kv4_head_bytes(hd)}], 16-byte aligned")
-    _req(block_table.dim() == 2 and block_table.dtype == torch.int32, f"{name}: block table int32 [slots, pages]")
+def _kv4_fail(name: str, why: str):
+    raise KernelError(f"{name}: {why}")
 
 
-def _same_device(name: str, *tensors) -> None:
-    """All on the current device: its stream is the one that the kernels are launched on."""
-    here = torch.cuda.current_device()
+# These calls take longer on the host than the smallest of them on the GPU: checks ask torch for as little as they can (a size, not a
+# shape; the device's number, which says at once that a tensor is on the GPU and on the current one), and messages are put
+# together only where one is needed (8 rows written and read back: 19.2 us a pass before, 16.4 now; their kernels take 5.3).
+def _kv4_here(name: str, *tensors) -> None:
+    """Every tensor dense and on the current device, whose stream the kernels are launched on."""
+    if not tensors[0].is_cuda:
+        raise KernelError(f"{name}: tensor on {tensors[0].device}; kernels run on the GPU only")
+    here = _current_device()
     for t in tensors:
-        if t is not None and t.device.index != here:
+        if t is None:
+            continue
+        if t.get_device() != here:
+            if not t.is_cuda:
+                raise KernelError(f"{name}: tensor on {t.device}; kernels run on the GPU only")
             raise KernelError(f"{name}: tensor on {t.device}, the current device is cuda:{here}")
+        if not t.is_contiguous():
+            raise KernelError(f"{name}: tensor of shape {tuple(t.shape)} is not contiguous")
+
+
+def _kv4_cache(name: str, cache: torch.Tensor, block_table: torch.Tensor, nkv: int, hd: int, page: int) -> None:
+    if page != KV4_PAGE:
+        _kv4_fail(name, f"pages of {KV4_PAGE} tokens")
+    if not (nkv > 0 and cache.dtype is torch.uint8 and cache.dim() == 3 and cache.size(1) == nkv and cache.size(2) == kv4_head_bytes(hd)
+            and cache.data_ptr() % 16 == 0):
+        _kv4_fail(name, f"cache unit must be uint8 [pages, nkv, {kv4_head_bytes(hd)}], 16-byte aligned")
+    if block_table.dim() != 2 or block_table.dtype is not torch.int32:
+        _kv4_fail(name, "block table int32 [slots, pages]")
 
 
 def _kv4_rows(name: str, positions, seq_of_token, slots, T: int) -> None:
-    _dev(name, positions, seq_of_token, slots)
-    _req(positions.dtype == seq_of_token.dtype == slots.dtype == torch.int32, f"{name}: positions, seq_of_token and slots must be int32")
-    _req(positions.numel() >= T and seq_of_token.numel() >= T, f"{name}: positions shorter than tokens")
+    if not (positions.dtype is torch.int32 and seq_of_token.dtype is torch.int32 and slots.dtype is torch.int32):
+        _kv4_fail(name, "positions, seq_of_token and slots must be int32")
+    if positions.numel() < T or seq_of_token.numel() < T:
+        _kv4_fail(name, "positions shorter than tokens")
+
+
+_KV4_WRITE = [_P, c_int, _P, _P, _P, _P, _P, c_int, _P, c_int, c_int, _P] + [c_int] * 8 + [_P]
+_KV4_READ = [_P, _P, c_int, _P, _P, _P, c_int, _P, c_int, c_int, _P] + [c_int] * 4 + [_P]
+_KV4_DECODE = [_P, c_size_t, _P, _P, _P, _P, c_int, c_int, _P] + [c_int] * 6 + [c_float, c_int, _P, _P, _P]
+_KV4_PREFILL = [_P, c_size_t, _P, _P, _P, _P, _P, c_int, c_int, _P] + [c_int] * 8 + [c_float, c_int, _P, _P, _P]
 
 
 def rope_kv4_write(qkv: torch.Tensor, cos: Optional[torch.Tensor], sin: Optional[torch.Tensor], positions: torch.Tensor,
@@ -1911,25 +1935,37 @@ def rope_kv4_write(qkv: torch.Tensor, cos: Optional[torch.Tensor], sin: Optional
     place, and puts rotated keys (rounded to the rows' type first) and values into their pages.  No two tokens of a step may
     stand at the same place of one slot."""
     name = "rope_kv4_write"
-    _dev(name, qkv, cos, sin)
-    _req(qkv.dim() == 2 and nq >= 0 and qkv.shape[1] == (nq + 2 * nkv) * hd, f"{name}: qkv width is not (nq + 2 nkv) * head_dim")
-    _req(qkv.data_ptr() % 16 == 0, f"{name}: rows must be 16-byte aligned")
-    T = qkv.shape[0]
+    _kv4_here(name, qkv, positions, seq_of_token, slots, block_table, cos, sin, cache)
+    if qkv.dim() != 2 or nq < 0 or qkv.size(1) != (nq + 2 * nkv) * hd:
+        _kv4_fail(name, "qkv width is not (nq + 2 nkv) * head_dim")
+    at = qkv.data_ptr()
+    if at % 16:
+        _kv4_fail(name, "rows must be 16-byte aligned")
+    T = qkv.size(0)
     _kv4_rows(name, positions, seq_of_token, slots, T)
     kv4_head_bytes(hd)
-    _req((cos is None) == (sin is None), f"{name}: both rotary tables, or none")
+    if (cos is None) != (sin is None):
+        _kv4_fail(name, "both rotary tables, or none")
     if cos is not None:
-        _req(0 <= rotary_dim <= hd and rotary_dim % 2 == 0, f"{name}: rotary_dim {rotary_dim} must be even, at most {hd}")
-        _req(cos.dtype == sin.dtype == torch.float32 and min(cos.numel(), sin.numel()) >= T * (rotary_dim // 2)
-             and cos.data_ptr() % 16 == 0 and sin.data_ptr() % 16 == 0, f"{name}: rotary tables must be float32 [T, rotary_dim / 2]")
+        if not 0 <= rotary_dim <= hd or rotary_dim % 2:
+            _kv4_fail(name, f"rotary_dim {rotary_dim} must be even, at most {hd}")
+        if not (cos.dtype is torch.float32 and sin.dtype is torch.float32 and min(cos.numel(), sin.numel()) >= T * (rotary_dim // 2)
+                and cos.data_ptr() % 16 == 0 and sin.data_ptr() % 16 == 0):
+            _kv4_fail(name, "rotary tables must be float32 [T, rotary_dim / 2], 16-byte aligned")
+    pages = 0
     if write_cache:
-        _req(cache is not None, f"{name}: no cache to write to")
+        if cache is None:
+            _kv4_fail(name, "no cache to write to")
         _kv4_cache(name, cache, block_table, nkv, hd, page)
-    _same_device(name, qkv, cos, sin, positions, seq_of_token, slots, block_table, cache)
-    f = _fn("kv4_cache", "br_rope_kv4_write", [_P, c_int, _P, _P, _P, _P, _P, c_int, _P, c_int, c_int, _P] + [c_int] * 8 + [_P])
-    _check(f(_ptr(qkv), _is_bf16(qkv, name), _ptr(cos), _ptr(sin), _ptr(positions), _ptr(seq_of_token), _ptr(slots), slots.numel(),
-             _ptr(block_table), block_table.shape[0], block_table.shape[1], _ptr(cache), cache.shape[0] if cache is not None else 0, T,
-             nq, nkv, hd, rotary_dim if cos is not None else 0, int(adjacent), int(write_cache), _stream()), name)
+        pages = cache.size(0)
+    elif block_table.dim() != 2:
+        _kv4_fail(name, "block table int32 [slots, pages]")
+    f = _fns.get(("kv4_cache", "br_rope_kv4_write")) or _fn("kv4_cache", "br_rope_kv4_write", _KV4_WRITE)
+    rc = f(at, _is_bf16(qkv, name), _ptr(cos), _ptr(sin), positions.data_ptr(), seq_of_token.data_ptr(), slots.data_ptr(), slots.numel(),
+           block_table.data_ptr(), block_table.size(0), block_table.size(1), _ptr(cache), pages, T, nq, nkv, hd,
+           rotary_dim if cos is not None else 0, int(adjacent), int(write_cache), _stream())
+    if rc:
+        _check(rc, name)
 
 
 def kv4_read(k_out: torch.Tensor, v_out: torch.Tensor, positions: torch.Tensor, seq_of_token: torch.Tensor, slots: torch.Tensor,
@@ -1937,17 +1973,20 @@ def kv4_read(k_out: torch.Tensor, v_out: torch.Tensor, positions: torch.Tensor, 
     """k_out[t], v_out[t] [T, nkv * hd] = what the cache holds for position positions[t] of sequence seq_of_token[t], exactly
     (bfloat16 or float32).  Rows of padding sequences (slot -1) are left as they are."""
     name = "kv4_read"
-    _dev(name, k_out, v_out)
-    _req(k_out.dim() == 2 and k_out.shape == v_out.shape and k_out.shape[1] == nkv * hd and k_out.dtype == v_out.dtype,
-         f"{name}: k_out and v_out must be [T, nkv * hd] of one type")
-    _req(k_out.data_ptr() % 16 == 0 and v_out.data_ptr() % 16 == 0, f"{name}: rows must be 16-byte aligned")
-    T = k_out.shape[0]
+    _kv4_here(name, k_out, v_out, positions, seq_of_token, slots, block_table, cache)
+    T = k_out.size(0) if k_out.dim() == 2 else -1
+    if T < 0 or v_out.dim() != 2 or v_out.size(0) != T or k_out.size(1) != nkv * hd or v_out.size(1) != nkv * hd or k_out.dtype is not v_out.dtype:
+        _kv4_fail(name, "k_out and v_out must be [T, nkv * hd] of one type")
+    k_at, v_at = k_out.data_ptr(), v_out.data_ptr()
+    if k_at % 16 or v_at % 16:
+        _kv4_fail(name, "rows must be 16-byte aligned")
     _kv4_rows(name, positions, seq_of_token, slots, T)
     _kv4_cache(name, cache, block_table, nkv, hd, page)
-    _same_device(name, k_out, v_out, positions, seq_of_token, slots, block_table, cache)
-    f = _fn("kv4_cache", "br_kv4_read", [_P, _P, c_int, _P, _P, _P, c_int, _P, c_int, c_int, _P] + [c_int] * 4 + [_P])
-    _check(f(_ptr(k_out), _ptr(v_out), _is_bf16(k_out, name), _ptr(positions), _ptr(seq_of_token), _ptr(slots), slots.numel(),
-             _ptr(block_table), block_table.shape[0], block_table.shape[1], _ptr(cache), cache.shape[0], T, nkv, hd, _stream()), name)
+    f = _fns.get(("kv4_cache", "br_kv4_read")) or _fn("kv4_cache", "br_kv4_read", _KV4_READ)
+    rc = f(k_at, v_at, _is_bf16(k_out, name), positions.data_ptr(), seq_of_token.data_ptr(), slots.data_ptr(), slots.numel(),
+           block_table.data_ptr(), block_table.size(0), block_table.size(1), cache.data_ptr(), cache.size(0), T, nkv, hd, _stream())
+    if rc:
+        _check(rc, name)
 
 
 def attention_kv4_splits(n_seqs: int, max_new: int, nq: int, nkv: int, hd: int, max_ctx: int, window: Optional[int] = None) -> int:
@@ -1975,27 +2014,38 @@ def attention_kv4_splits(n_seqs: int, max_new: int, nq: int, nkv: int, hd: int, 
     return max(1, min(64, cus // groups, pages // 8))
 
 
-def _attention_kv4(name, q, out, slots, ctx_lens, block_table, cache, B, T, nq, nkv, hd, page, window, scale, nsplit, part_o, part_ml, more=()):
-    _dev(name, out, slots, ctx_lens, part_o, part_ml, *more)
-    _req(q.is_cuda and q.dtype == torch.bfloat16 and out.dtype == torch.bfloat16, f"{name}: bfloat16 only")
+def _attention_kv4(name, q, q_stride, out, slots, ctx_lens, block_table, cache, B, T, nq, nkv, hd, page, window, scale, nsplit, part_o, part_ml) -> None:
+    bf16 = torch.bfloat16
+    if q.dtype is not bf16 or out.dtype is not bf16:
+        _kv4_fail(name, "bfloat16 only")
     _kv4_cache(name, cache, block_table, nkv, hd, page)
-    _req(nq > 0 and nq % nkv == 0 and out.dim() == 2 and out.shape[1] == nq * hd and out.shape[0] >= T, f"{name}: out must be [T, nq * hd]")
-    _req(slots.dtype == ctx_lens.dtype == torch.int32 and min(slots.numel(), ctx_lens.numel()) >= B, f"{name}: slots and ctx_lens int32 [B]")
-    _req(scale > 0, f"{name}: the score scale must be positive, not {scale} (the kernels take the row maximum before scaling)")
-    _req(window is None or window > 0, f"{name}: the window must be positive or None, not {window}")
-    _req(1 <= nsplit <= 64, f"{name}: 1 to 64 runs, not {nsplit}")
-    if nsplit > 1:
-        _req(part_o is not None and part_ml is not None and part_o.dtype == part_ml.dtype == torch.float32
-             and part_o.numel() >= T * nq * nsplit * hd and part_ml.numel() >= T * nq * nsplit * 2 and part_o.data_ptr() % 16 == 0,
-             f"{name}: scratch for the runs is too small")
-    _same_device(name, q, out, slots, ctx_lens, block_table, cache, part_o, part_ml, *more)
+    if nq <= 0 or nq % nkv or out.dim() != 2 or out.size(1) != nq * hd or out.size(0) < T:
+        _kv4_fail(name, "out must be [T, nq * hd]")
+    if not (slots.dtype is torch.int32 and ctx_lens.dtype is torch.int32 and slots.numel() >= B and ctx_lens.numel() >= B):
+        _kv4_fail(name, "slots and ctx_lens int32 [B]")
+    if not scale > 0:
+        _kv4_fail(name, f"the score scale must be positive, not {scale} (the kernels take the row maximum before scaling)")
+    if window is not None and window <= 0:
+        _kv4_fail(name, f"the window must be positive or None, not {window}")
+    if nsplit != 1:
+        if not 1 <= nsplit <= 64:
+            _kv4_fail(name, f"1 to 64 runs, not {nsplit}")
+        if not (part_o is not None and part_ml is not None and part_o.dtype is torch.float32 and part_ml.dtype is torch.float32
+                and part_o.numel() >= T * nq * nsplit * hd and part_ml.numel() >= T * nq * nsplit * 2 and part_o.data_ptr() % 16 == 0):
+            _kv4_fail(name, "scratch for the runs is too small")
+    # q's storage holds T rows of nq * hd elements, q_stride apart, from its first element on
+    width = nq * hd
+    if q_stride < width or q_stride % 8 or q.data_ptr() % 16:
+        _kv4_fail(name, "query rows must be 16-byte aligned")
+    rows = (T - 1) * q_stride + width
+    if T > 0 and rows > q.numel() and rows > q.untyped_storage().nbytes() // 2 - q.storage_offset():
+        _kv4_fail(name, f"q holds fewer than {T} rows of {width}, {q_stride} apart")
 
 
-def _q_rows(name: str, q: torch.Tensor, q_stride: int, T: int, width: int) -> None:
-    """`q`'s storage holds T rows of `width` elements, `q_stride` apart, from its first element on."""
-    _req(q_stride >= width and q_stride % 8 == 0 and q.data_ptr() % 16 == 0, f"{name}: query rows must be 16-byte aligned")
-    room = q.untyped_storage().nbytes() // q.element_size() - q.storage_offset()
-    _req(T == 0 or (T - 1) * q_stride + width <= room, f"{name}: q holds fewer than {T} rows of {width}, {q_stride} apart")
+def _kv4_q_here(name: str, q: torch.Tensor, out: torch.Tensor) -> None:
+    """Queries may be columns of wider rows: on the device of the others, dense or not."""
+    if q.get_device() != out.get_device():
+        _kv4_fail(name, f"queries on {q.device}, the output on {out.device}")
 
 
 def attention_decode_kv4(q: torch.Tensor, q_stride: int, out: torch.Tensor, slots: torch.Tensor, ctx_lens: torch.Tensor,
@@ -2006,13 +2056,14 @@ def attention_decode_kv4(q: torch.Tensor, q_stride: int, out: torch.Tensor, slot
     already (`rope_kv4_write`).  Rows of padding sequences, and of sequences of no tokens, are zero.  `nsplit`:
     `attention_kv4_splits`.  Two calls that may run at the same time need scratch of their own."""
     name = "attention_decode_kv4"
-    _attention_kv4(name, q, out, slots, ctx_lens, block_table, cache, B, B, nq, nkv, hd, page, window, scale, nsplit, part_o, part_ml)
-    _q_rows(name, q, q_stride, B, nq * hd)
-    f = _fn("attention_kv4", "br_attn_decode_kv4",
-            [_P, c_size_t, _P, _P, _P, _P, c_int, c_int, _P] + [c_int] * 6 + [c_float, c_int, _P, _P, _P])
-    _check(f(_ptr(q), q_stride, _ptr(out), _ptr(slots), _ptr(ctx_lens), _ptr(block_table), block_table.shape[0], block_table.shape[1],
-             _ptr(cache), cache.shape[0], B, nq, nkv, hd, int(window or 0), float(scale), nsplit, _ptr(part_o), _ptr(part_ml), _stream()),
-           name)
+    _kv4_here(name, out, slots, ctx_lens, block_table, cache, part_o, part_ml)
+    _kv4_q_here(name, q, out)
+    _attention_kv4(name, q, q_stride, out, slots, ctx_lens, block_table, cache, B, B, nq, nkv, hd, page, window, scale, nsplit, part_o, part_ml)
+    f = _fns.get(("attention_kv4", "br_attn_decode_kv4")) or _fn("attention_kv4", "br_attn_decode_kv4", _KV4_DECODE)
+    rc = f(q.data_ptr(), q_stride, out.data_ptr(), slots.data_ptr(), ctx_lens.data_ptr(), block_table.data_ptr(), block_table.size(0),
+           block_table.size(1), cache.data_ptr(), cache.size(0), B, nq, nkv, hd, min(window or 0, 0x7fffffff), scale, nsplit, _ptr(part_o), _ptr(part_ml), _stream())
+    if rc:
+        _check(rc, name)
 
 
 def attention_prefill_kv4(q: torch.Tensor, q_stride: int, out: torch.Tensor, cu_seqlens: torch.Tensor, slots: torch.Tensor,
@@ -2021,19 +2072,23 @@ def attention_prefill_kv4(q: torch.Tensor, q_stride: int, out: torch.Tensor, cu_
                           part_o: Optional[torch.Tensor] = None, part_ml: Optional[torch.Tensor] = None) -> None:
     """`attention_prefill_bf16` over a cache of 4-bit keys and values, which holds the new tokens already (`rope_kv4_write`):
     sequence b's are rows cu_seqlens[b] .. cu_seqlens[b + 1] of `out` and `q`, the last of its ctx_lens[b] tokens; `max_new` is
-    the most of one sequence.  Rows of padding sequences are zero, rows behind the last sequence stay as they are."""
+    the most of one sequence.  Rows of padding sequences are zero, rows behind the last sequence stay as they are.  `nsplit`:
+    `attention_kv4_splits`.  Two calls that may run at the same time need scratch of their own."""
     name = "attention_prefill_kv4"
-    T = out.shape[0]
-    _attention_kv4(name, q, out, slots, ctx_lens, block_table, cache, B, T, nq, nkv, hd, page, window, scale, nsplit, part_o, part_ml,
-                   (cu_seqlens,))
-    _q_rows(name, q, q_stride, T, nq * hd)
-    _req(cu_seqlens.dtype == torch.int32 and cu_seqlens.numel() >= B + 1, f"{name}: cu_seqlens int32 [B + 1]")
-    _req(0 <= max_new <= T, f"{name}: max_new {max_new} of {T} rows")
-    f = _fn("attention_kv4", "br_attn_prefill_kv4",
-            [_P, c_size_t, _P, _P, _P, _P, _P, c_int, c_int, _P] + [c_int] * 8 + [c_float, c_int, _P, _P, _P])
-    _check(f(_ptr(q), q_stride, _ptr(out), _ptr(cu_seqlens), _ptr(slots), _ptr(ctx_lens), _ptr(block_table), block_table.shape[0],
-             block_table.shape[1], _ptr(cache), cache.shape[0], B, max_new, T, nq, nkv, hd, int(window or 0), float(scale), nsplit,
-             _ptr(part_o), _ptr(part_ml), _stream()), name)
+    _kv4_here(name, out, cu_seqlens, slots, ctx_lens, block_table, cache, part_o, part_ml)
+    _kv4_q_here(name, q, out)
+    T = out.size(0)
+    _attention_kv4(name, q, q_stride, out, slots, ctx_lens, block_table, cache, B, T, nq, nkv, hd, page, window, scale, nsplit, part_o, part_ml)
+    if cu_seqlens.dtype is not torch.int32 or cu_seqlens.numel() < B + 1:
+        _kv4_fail(name, "cu_seqlens int32 [B + 1]")
+    if not 0 <= max_new <= T:
+        _kv4_fail(name, f"max_new {max_new} of {T} rows")
+    f = _fns.get(("attention_kv4", "br_attn_prefill_kv4")) or _fn("attention_kv4", "br_attn_prefill_kv4", _KV4_PREFILL)
+    rc = f(q.data_ptr(), q_stride, out.data_ptr(), cu_seqlens.data_ptr(), slots.data_ptr(), ctx_lens.data_ptr(), block_table.data_ptr(),
+           block_table.size(0), block_table.size(1), cache.data_ptr(), cache.size(0), B, max_new, T, nq, nkv, hd, min(window or 0, 0x7fffffff), scale, nsplit,
+           _ptr(part_o), _ptr(part_ml), _stream())
+    if rc:
+        _check(rc, name)
 
 
 # -------------------------------------------------------------------- sampling -----
