@@ -149,7 +149,11 @@ def with_kv_cache(spec: ModelSpec, held: Optional[str]) -> ModelSpec:
     kinds = {m.kind for ls in spec.layers for m in [ls.mixer, *ls.more_mixers.values()] if m is not None}
     if kinds - {"gqa_attention"}:
         raise ConfigError(f"kv_cache {held!r} is built for models whose mixers are gqa_attention; {spec.architecture} has {sorted(kinds)}")
-    layers = [ls if ls.mixer is None else replace(ls, mixer=PartSpec(ls.mixer.kind, {**ls.mixer.params, "kv_cache": held})) for ls in spec.layers]
+
+    def so_held(mixer: Optional[PartSpec]) -> Optional[PartSpec]:
+        return None if mixer is None else PartSpec(mixer.kind, {**mixer.params, "kv_cache": held})
+
+    layers = [replace(ls, mixer=so_held(ls.mixer), more_mixers={role: so_held(m) for role, m in ls.more_mixers.items()}) for ls in spec.layers]
     return replace(spec, layers=layers)
 
 

@@ -103,6 +103,18 @@ def test_models_that_can_hold_keys_and_values_in_4_bits():
         GQAAttention(64, 2, 1, 32, kv_cache="mxfp8")
 
 
+def test_mixers_side_by_side_are_both_held_in_4_bits():
+    from dataclasses import replace
+    import braidinfer_amd as B
+    from braidinfer_amd.config import LayerSpec, PartSpec, spec_of, with_kv_cache
+    mixer = PartSpec("gqa_attention", {"hidden_size": 64, "num_heads": 2, "num_kv_heads": 1, "head_dim": 32})
+    spec = replace(spec_of(B.preset("mistral-7b-v0.1", num_hidden_layers=2)),
+                   layers=[LayerSpec(prefix="a."), LayerSpec(prefix="b.", mixer=mixer, more_mixers={"right": mixer})])
+    got = with_kv_cache(spec, "mxfp4").layers
+    assert got[0].mixer is None and got[1].mixer.params["kv_cache"] == got[1].more_mixers["right"].params["kv_cache"] == "mxfp4"
+    assert "kv_cache" not in mixer.params
+
+
 def test_units_held_in_4_bits():
     from braidinfer_amd.cache import CacheNeed, SequenceCache
     from braidinfer_amd.errors import CacheError
