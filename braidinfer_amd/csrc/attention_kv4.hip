@@ -447,9 +447,10 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(M <= 4 && G
     int x = 0, end = 0;                                 // this workgroup's places of the list
     if (pieces) {
         list.start(runs, seqs, lane);
-        x = (int)blockIdx.x * list.p;
-        const int all = list.total * runs.groups;
-        end = x + list.p < all ? x + list.p : all;
+        const int all = list.total * runs.groups;       // below 2^30; shares that begin behind it may begin behind 2^31 as well
+        const long long from = (long long)blockIdx.x * list.p;
+        x = from < all ? (int)from : all;
+        end = all - x > list.p ? x + list.p : all;
         // sequences of no tokens are in nobody's part
         for (int from = blockIdx.x * WAVE; from < runs.B; from += gridDim.x * WAVE) {
             Kv4List some = list;
