@@ -671,6 +671,7 @@ __global__ __launch_bounds__(256) void attn_kv4_join_kernel(const float* __restr
 // Several tokens per sequence.  A workgroup takes `tile_rows` <= 32 NW rows of one kv head and sequence, row = token * G + head, 32 a wave, and
 // walks the pages that they see.  A page's codes come to registers while the page before is multiplied, are turned into
 // bfloat16 once for all waves and lie in LDS in the order of the matrix operands, 1 KB a wave-read, two pages deep; one barrier a page.
+// KH 2: a row has two waves, one for each half of every page, joined at the end: half as many rows, and a page in 1.7 us instead of 2.5.
 // Chunk [half][k-step][lane] of the keys: 8 channels of the key that row lane % 32 of a 32-key block stands for.  Chunk [32 channels]
 // [16 tokens][lane] of the values: 8 tokens of a channel.  (A code and its scale become bfloat16 in half an instruction; read by
 // every wave for itself they would cost NW times as many.)
@@ -682,13 +683,13 @@ __device__ __forceinline__ int kv4_row_of_key(int u) { return (u & 3) | (((u >> 
 // Place of a channel's row among a value chunk's 32: turned so that the 16 lanes that write different rows at a time reach different banks
 __device__ __forceinline__ int kv4_value_row(int row, int i2) { return row ^ ((row >> 4) | ((i2 & 3) << 1)); }
 
-template <int M, int NW>
-__global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(NW == 4 && M > 4 ? 1 : 2, 2))) void attn_prefill_kv4_kernel(const bf16* __restrict__ q, size_t q_stride, bf16* __restrict__ out,
+template <int M, int NW, int KH>
+__global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(M > 4 ? 1 : M <= 2 ? 4 : 2, M <= 2 ? 4 : 2))) void attn_prefill_kv4_kernel(const bf16* __restrict__ q, size_t q_stride, bf16* __restrict__ out,
                                                                    const int* __restrict__ cu_seqlens, Kv4Seqs seqs,
                                                                    const unsigned char* __restrict__ cache, int nq, int nkv, int window,
                                                                    float scale, const PrefillOrder order, int n_tokens, int tile_rows, int nsplit,
                                                                    float* __restrict__ part_o, float* __restrict__ part_ml) {
-    constexpr int HD = 32 * M, NT = NW * 64;
+    constexpr int HD = 32 * M, NT = NW * 64, RW = NW / KH;
     constexpr int KB = KV4_PAGE * HD * 2, STAGE = 2 * KB;                       // bytes of a page's keys; keys and values
     constexpr int UNITS = 64 * M, UPT = (UNITS + NT - 1) / NT;                    // units of 32 elements of the keys, as many of the values; of each a thread
     typedef kv4_layout<M> L;
@@ -707,7 +708,8 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(NW == 4
     const long long rows_total = (long long)n_new * G;
     if (t0 < 0 || t0 + n_new > n_tokens || (long long)tile * tile_rows >= rows_total) return;        // the whole workgroup leaves together
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int row0 = tile * tile_rows + wave * 32;
+    const int rw = KH == 1 ? wave : wave % RW, kh = KH == 1 ? 0 : wave / RW;   // the wave's 32 rows and, of KH 2, its half of every page
+    const int row0 = tile * tile_rows + rw * 32;
     const int c = lane & 31, g = lane >> 5;
     const int last = (int)(rows_total < (long long)(tile + 1) * tile_rows ? rows_total : (long long)(tile + 1) * tile_rows) - 1;       // of the tile's
     const bool wave_ok = row0 <= last, row_ok = row0 + c <= last;
@@ -752,7 +754,9 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(NW == 4
     auto value_half = [](int u) { return M % 4 == 0 ? (u >> 4) & 1 : u / (32 * M); };
     auto value_tg = [](int u) { return M % 4 == 0 ? (u >> 5) & 7 : u / (4 * M) & 7; };
     // Waves without rows, the last ones, convert where a tile has such; the first ones in full tiles (8,192 tokens: 547 us against 585 by the last).
-    const int unit0 = (tile_rows < 32 * NW ? NW - 1 - wave : wave) * 64 + lane;
+    const int with_rows = tile_rows / 32;
+    const int turn = KH == 1 ? (with_rows < NW ? NW - 1 - wave : wave) : rw >= with_rows ? (rw - with_rows) * 2 + kh : 2 * (RW - with_rows) + kh * with_rows + rw;
+    const int unit0 = turn * 64 + lane;
     u32x4 kr[UPT], va[UPT], vb[UPT];
     u32x2 vsr[UPT];
     unsigned ksr[UPT];
@@ -932,14 +936,42 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(NW == 4
         const int kb = pi * KV4_PAGE;
         const bool s0 = wave_ok && kb <= pq_max_w && (window <= 0 || kb + 31 > pq_min_w - window);
         const bool s1 = wave_ok && kb + 32 <= pq_max_w && (window <= 0 || kb + 63 > pq_min_w - window);
-        if (s0) block(0);
-        if (s1) block(1);
+        if constexpr (KH == 1) {
+            if (s0) block(0);
+            if (s1) block(1);
+        } else if (kh ? s1 : s0) block(kh);
         bring();
         kv4_lds_barrier();
         pi = pn;
         pn = pm;
     }
     l += __shfl_xor(l, 32, WAVE);
+    if constexpr (KH == 2) {
+        // the second half's sums go to the wave of the same rows through LDS, where no page is needed any more
+        f32x4* const theirs = (f32x4*)dsm + (size_t)rw * (4 * M * 64) + lane;
+        float* const ml = (float*)(dsm + (size_t)RW * M * 4096) + rw * 128 + lane;
+        if (kh) {
+#pragma unroll
+            for (int i = 0; i < M; ++i)
+#pragma unroll
+                for (int r4 = 0; r4 < 4; ++r4) theirs[(4 * i + r4) * 64] = f32x4{o[i][4 * r4], o[i][4 * r4 + 1], o[i][4 * r4 + 2], o[i][4 * r4 + 3]};
+            ml[0] = m;
+            ml[64] = l;
+        }
+        __syncthreads();
+        if (kh) return;
+        const float m1 = ml[0], l1 = ml[64], both = fmaxf(m, m1), use = both == -INFINITY ? 0.f : both, f0 = kv4_exp2(m - use), f1 = kv4_exp2(m1 - use);
+        m = both;
+        l = l * f0 + l1 * f1;
+#pragma unroll
+        for (int i = 0; i < M; ++i)
+#pragma unroll
+            for (int r4 = 0; r4 < 4; ++r4) {
+                const f32x4 x = theirs[(4 * i + r4) * 64];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) o[i][4 * r4 + e] = o[i][4 * r4 + e] * f0 + x[e] * f1;
+            }
+    }
     if (!row_ok) return;
     const float inv = nsplit > 1 ? 1.f : l == 0.f ? 0.f : 1.f / l;
     const size_t at = nsplit > 1 ? orow * nsplit + split : orow;
@@ -1018,10 +1050,15 @@ extern "C" int br_attn_prefill_kv4(const void* q, size_t q_stride, void* out, co
     const long long rows = (long long)max_new * (nq / nkv);
     if (rows > 0x7fffffffLL - 256) return BR_BAD_ARG;
     if (B == 0 || max_new == 0) return BR_OK;
-    // 8 waves convert a page once for 256 rows.  4 waves, two workgroups to a compute unit, where 8 would leave units without one or
-    // the last tiles alone: a prompt of 67 tokens 9.0 us against 11.3, 512 25.7 / 28.4, 2,048 79 / 82, but 4,096 183 / 167, 8,192 666 / 615.
-    const int cus = br_device_cus() > 0 ? br_device_cus() : 256;
-    const bool wide = hd <= 128 && (nsplit > 1 || (rows + 255) / 256 * nkv * B > cus);      // larger heads have no registers for 8 waves
+    // 8 waves convert a page once for 256 rows.  Tiles of 128 rows, two waves to 32 of them and each with a half of every page, where 256 would
+    // leave units without a tile or a few long ones last: 128 tokens of 32 heads of 128 over 8 in 11.0 us, not 13.3, 512 19.2 / 24.6, 2,048
+    // 66 / 74, but 3,000 126 / 102; for several sequences, whose tiles differ less, earlier: twice 1,500 79 / 70, 8 times 250 26 / 23.  Of heads
+    // of up to 64 two workgroups share a unit (32 over 4 heads of 64: 2,000 tokens 47.8 / 58.0, 1,357 to 93 50 / 52, 16 times 500 56 / 43, 8,192 387 / 332).
+    // In runs: 5 tokens behind 3,800 of 8 users 33 / 40, 16 behind 16,000 23.3 / 24.6, 32 behind 16,352 29.3 / 28.1.
+    const int cus = br_device_cus() > 0 ? br_device_cus() : 256, each = hd <= 64 ? 2 : 1;
+    const long long filled = ((long long)n_tokens * (nq / nkv) + 255) / 256 * nkv;
+    // larger heads have no registers for 8 waves
+    const bool wide = hd <= 128 && (nsplit > 1 ? rows > 64 : filled > (each == 2 || B == 1 ? each * cus : cus / 2));
     const int most = wide ? 256 : 128;
     const long long tiles = (rows + most - 1) / most;
     PrefillOrder order = {};
@@ -1032,15 +1069,15 @@ extern "C" int br_attn_prefill_kv4(const void* q, size_t q_stride, void* out, co
         tile_rows = (int)(((rows + tiles - 1) / tiles + 31) / 32 * 32);
         if (tiles * nsplit > 0x7fffffffLL) return BR_BAD_ARG;
         grid = dim3((unsigned)(tiles * nsplit), nkv, B);
-    } else if (!prefill_order(order, grid, wide ? (rows + 1) / 2 : rows, nkv, B, cus, !wide && hd <= 128 ? 2 : 1)) return BR_BAD_ARG;   // it counts in tiles of 128
-    const size_t lds = 2 * (size_t)2 * KV4_PAGE * hd * 2 + 16 + 2 * (hd / 32) * 8;
+    } else if (!prefill_order(order, grid, wide ? (rows + 1) / 2 : rows, nkv, B, cus, each)) return BR_BAD_ARG;   // it counts in tiles of 128
+    const size_t lds = 2 * (size_t)2 * KV4_PAGE * hd * 2 + (!wide && hd <= 128 ? 4 * 128 * sizeof(float) : 16 + 2 * (hd / 32) * 8);
     const Kv4Seqs seqs = {slots, ctx_lens, table, n_slots, table_pages, n_pages};
-#define GO(M_, NW_) { \
+#define GO(M_, NW_, KH_) { \
         static unsigned long long told; \
-        if (lds > 65536 && !kv4_allow((const void*)attn_prefill_kv4_kernel<M_, NW_>, lds, told)) return BR_LAUNCH_FAILED; \
-        attn_prefill_kv4_kernel<M_, NW_><<<grid, NW_ * 64, lds, s>>>((const bf16*)q, q_stride, (bf16*)out, cu_seqlens, seqs, (const unsigned char*)cache, nq, nkv, window, scale, order, n_tokens, tile_rows, nsplit, part_o, part_ml); }
-#define CASE(M_) case M_: GO(M_, 4) break;
-#define BOTH(M_) case M_: if (wide) GO(M_, 8) else GO(M_, 4) break;
+        if (lds > 65536 && !kv4_allow((const void*)attn_prefill_kv4_kernel<M_, NW_, KH_>, lds, told)) return BR_LAUNCH_FAILED; \
+        attn_prefill_kv4_kernel<M_, NW_, KH_><<<grid, NW_ * 64, lds, s>>>((const bf16*)q, q_stride, (bf16*)out, cu_seqlens, seqs, (const unsigned char*)cache, nq, nkv, window, scale, order, n_tokens, tile_rows, nsplit, part_o, part_ml); }
+#define CASE(M_) case M_: GO(M_, 4, 1) break;
+#define BOTH(M_) case M_: if (wide) GO(M_, 8, 1) else GO(M_, 8, 2) break;
     switch (hd / 32) { BOTH(1) BOTH(2) BOTH(3) BOTH(4) CASE(5) CASE(6) CASE(7) CASE(8) }
 #undef BOTH
 #undef CASE

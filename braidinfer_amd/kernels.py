@@ -2008,8 +2008,10 @@ def attention_kv4_splits(n_seqs: int, max_new: int, nq: int, nkv: int, hd: int, 
             return 1
         # the most pieces of a sequence that the scratch holds: eight times its even share, as one that is longer than the others has
         return max(2, min(64, -(-pages // 4) + 1, 2 + 24 * cus // max(1, groups)))
-    # tiles of 256 rows (128 for heads beyond 128) that leave compute units without work: as many runs as fill them once, of 8 pages at
-    # least (67 tokens behind 16,344: 608 us whole, 79 in 8 runs, 50 in 16, 73 in 20; 512 behind none 21 us whole, 28 in 2 runs)
+    # tiles of 256 rows (128 for heads beyond 128) that leave compute units without work: as many runs as fill them once, of 8 of the
+    # pages that a row sees on average at least (67 tokens behind 16,344: 608 us whole, 79 in 8 runs, 50 in 16, 73 in 20; 512 behind
+    # none 19 us whole, 28 in 2 runs)
+    pages -= max_new // 2 // KV4_PAGE
     groups = max(1, n_seqs * nkv * -(-(max_new * (nq // nkv)) // (256 if hd <= 128 else 128)))
     return max(1, min(64, cus // groups, pages // 8))
 
