@@ -1886,9 +1886,10 @@ def _kv4_fail(name: str, why: str):
     raise KernelError(f"{name}: {why}")
 
 
-# These calls take longer on the host than the smallest of them on the GPU: checks ask torch for as little as they can (a size, not a
-# shape; the device's number, which says at once that a tensor is on the GPU and on the current one), and messages are put
-# together only where one is needed (8 rows written and read back: 19.2 us a pass before, 16.4 now; their kernels take 5.3).
+# These calls take longer on the host than the smallest of them on the GPU: checks ask torch for as little as they can (a shape
+# once, not its sizes; the device's number, which says at once that a tensor is on the GPU and on the current one), and messages are put
+# together only where one is needed (8 rows written and read back: 19.2 us a pass before, 15.5 now; their kernels take 5.3, two launches
+# alone 8.1).
 def _kv4_here(name: str, *tensors) -> None:
     """Every tensor dense and on the current device, whose stream the kernels are launched on."""
     if not tensors[0].is_cuda:
@@ -1905,14 +1906,21 @@ def _kv4_here(name: str, *tensors) -> None:
             raise KernelError(f"{name}: tensor of shape {tuple(t.shape)} is not contiguous")
 
 
-def _kv4_cache(name: str, cache: torch.Tensor, block_table: torch.Tensor, nkv: int, hd: int, page: int) -> None:
+def _kv4_cache(name: str, cache: torch.Tensor, block_table: torch.Tensor, nkv: int, hd: int, page: int):
+    """The pages of the cache, the rows and columns of the table."""
     if page != KV4_PAGE:
         _kv4_fail(name, f"pages of {KV4_PAGE} tokens")
-    if not (nkv > 0 and cache.dtype is torch.uint8 and cache.dim() == 3 and cache.size(1) == nkv and cache.size(2) == kv4_head_bytes(hd)
-            and cache.data_ptr() % 16 == 0):
+    shape = cache.shape
+    if not (nkv > 0 and cache.dtype is torch.uint8 and len(shape) == 3 and shape[1:] == (nkv, kv4_head_bytes(hd)) and cache.data_ptr() % 16 == 0):
         _kv4_fail(name, f"cache unit must be uint8 [pages, nkv, {kv4_head_bytes(hd)}], 16-byte aligned")
-    if block_table.dim() != 2 or block_table.dtype is not torch.int32:
+    return (shape[0], *_kv4_table(name, block_table))
+
+
+def _kv4_table(name: str, block_table: torch.Tensor):
+    shape = block_table.shape
+    if len(shape) != 2 or block_table.dtype is not torch.int32:
         _kv4_fail(name, "block table int32 [slots, pages]")
+    return shape
 
 
 def _kv4_rows(name: str, positions, seq_of_token, slots, T: int) -> None:
@@ -1936,12 +1944,13 @@ def rope_kv4_write(qkv: torch.Tensor, cos: Optional[torch.Tensor], sin: Optional
     stand at the same place of one slot."""
     name = "rope_kv4_write"
     _kv4_here(name, qkv, positions, seq_of_token, slots, block_table, cos, sin, cache)
-    if qkv.dim() != 2 or nq < 0 or qkv.size(1) != (nq + 2 * nkv) * hd:
+    shape = qkv.shape
+    if len(shape) != 2 or nq < 0 or shape[1] != (nq + 2 * nkv) * hd:
         _kv4_fail(name, "qkv width is not (nq + 2 nkv) * head_dim")
     at = qkv.data_ptr()
     if at % 16:
         _kv4_fail(name, "rows must be 16-byte aligned")
-    T = qkv.size(0)
+    T = shape[0]
     _kv4_rows(name, positions, seq_of_token, slots, T)
     kv4_head_bytes(hd)
     if (cos is None) != (sin is None):
@@ -1952,17 +1961,15 @@ def rope_kv4_write(qkv: torch.Tensor, cos: Optional[torch.Tensor], sin: Optional
         if not (cos.dtype is torch.float32 and sin.dtype is torch.float32 and min(cos.numel(), sin.numel()) >= T * (rotary_dim // 2)
                 and cos.data_ptr() % 16 == 0 and sin.data_ptr() % 16 == 0):
             _kv4_fail(name, "rotary tables must be float32 [T, rotary_dim / 2], 16-byte aligned")
-    pages = 0
     if write_cache:
         if cache is None:
             _kv4_fail(name, "no cache to write to")
-        _kv4_cache(name, cache, block_table, nkv, hd, page)
-        pages = cache.size(0)
-    elif block_table.dim() != 2:
-        _kv4_fail(name, "block table int32 [slots, pages]")
+        pages, n_slots, table_pages = _kv4_cache(name, cache, block_table, nkv, hd, page)
+    else:
+        pages, (n_slots, table_pages) = 0, _kv4_table(name, block_table)
     f = _fns.get(("kv4_cache", "br_rope_kv4_write")) or _fn("kv4_cache", "br_rope_kv4_write", _KV4_WRITE)
     rc = f(at, _is_bf16(qkv, name), _ptr(cos), _ptr(sin), positions.data_ptr(), seq_of_token.data_ptr(), slots.data_ptr(), slots.numel(),
-           block_table.data_ptr(), block_table.size(0), block_table.size(1), _ptr(cache), pages, T, nq, nkv, hd,
+           block_table.data_ptr(), n_slots, table_pages, _ptr(cache), pages, T, nq, nkv, hd,
            rotary_dim if cos is not None else 0, int(adjacent), int(write_cache), _stream())
     if rc:
         _check(rc, name)
@@ -1974,17 +1981,18 @@ def kv4_read(k_out: torch.Tensor, v_out: torch.Tensor, positions: torch.Tensor, 
     (bfloat16 or float32).  Rows of padding sequences (slot -1) are left as they are."""
     name = "kv4_read"
     _kv4_here(name, k_out, v_out, positions, seq_of_token, slots, block_table, cache)
-    T = k_out.size(0) if k_out.dim() == 2 else -1
-    if T < 0 or v_out.dim() != 2 or v_out.size(0) != T or k_out.size(1) != nkv * hd or v_out.size(1) != nkv * hd or k_out.dtype is not v_out.dtype:
+    shape = k_out.shape
+    if len(shape) != 2 or shape != v_out.shape or shape[1] != nkv * hd or k_out.dtype is not v_out.dtype:
         _kv4_fail(name, "k_out and v_out must be [T, nkv * hd] of one type")
+    T = shape[0]
     k_at, v_at = k_out.data_ptr(), v_out.data_ptr()
     if k_at % 16 or v_at % 16:
         _kv4_fail(name, "rows must be 16-byte aligned")
     _kv4_rows(name, positions, seq_of_token, slots, T)
-    _kv4_cache(name, cache, block_table, nkv, hd, page)
+    pages, n_slots, table_pages = _kv4_cache(name, cache, block_table, nkv, hd, page)
     f = _fns.get(("kv4_cache", "br_kv4_read")) or _fn("kv4_cache", "br_kv4_read", _KV4_READ)
     rc = f(k_at, v_at, _is_bf16(k_out, name), positions.data_ptr(), seq_of_token.data_ptr(), slots.data_ptr(), slots.numel(),
-           block_table.data_ptr(), block_table.size(0), block_table.size(1), cache.data_ptr(), cache.size(0), T, nkv, hd, _stream())
+           block_table.data_ptr(), n_slots, table_pages, cache.data_ptr(), pages, T, nkv, hd, _stream())
     if rc:
         _check(rc, name)
 
@@ -2016,12 +2024,14 @@ def attention_kv4_splits(n_seqs: int, max_new: int, nq: int, nkv: int, hd: int, 
     return max(1, min(64, cus // groups, pages // 8))
 
 
-def _attention_kv4(name, q, q_stride, out, slots, ctx_lens, block_table, cache, B, T, nq, nkv, hd, page, window, scale, nsplit, part_o, part_ml) -> None:
+def _attention_kv4(name, q, q_stride, out, slots, ctx_lens, block_table, cache, B, T, nq, nkv, hd, page, window, scale, nsplit, part_o, part_ml):
+    """The pages of the cache, the rows and columns of the table."""
     bf16 = torch.bfloat16
     if q.dtype is not bf16 or out.dtype is not bf16:
         _kv4_fail(name, "bfloat16 only")
-    _kv4_cache(name, cache, block_table, nkv, hd, page)
-    if nq <= 0 or nq % nkv or out.dim() != 2 or out.size(1) != nq * hd or out.size(0) < T:
+    sizes = _kv4_cache(name, cache, block_table, nkv, hd, page)
+    shape = out.shape
+    if nq <= 0 or nq % nkv or len(shape) != 2 or shape[1] != nq * hd or shape[0] < T:
         _kv4_fail(name, "out must be [T, nq * hd]")
     if not (slots.dtype is torch.int32 and ctx_lens.dtype is torch.int32 and slots.numel() >= B and ctx_lens.numel() >= B):
         _kv4_fail(name, "slots and ctx_lens int32 [B]")
@@ -2042,6 +2052,7 @@ def _attention_kv4(name, q, q_stride, out, slots, ctx_lens, block_table, cache, 
     rows = (T - 1) * q_stride + width
     if T > 0 and rows > q.numel() and rows > q.untyped_storage().nbytes() // 2 - q.storage_offset():
         _kv4_fail(name, f"q holds fewer than {T} rows of {width}, {q_stride} apart")
+    return sizes
 
 
 def _kv4_q_here(name: str, q: torch.Tensor, out: torch.Tensor) -> None:
@@ -2060,10 +2071,10 @@ def attention_decode_kv4(q: torch.Tensor, q_stride: int, out: torch.Tensor, slot
     name = "attention_decode_kv4"
     _kv4_here(name, out, slots, ctx_lens, block_table, cache, part_o, part_ml)
     _kv4_q_here(name, q, out)
-    _attention_kv4(name, q, q_stride, out, slots, ctx_lens, block_table, cache, B, B, nq, nkv, hd, page, window, scale, nsplit, part_o, part_ml)
+    pages, n_slots, table_pages = _attention_kv4(name, q, q_stride, out, slots, ctx_lens, block_table, cache, B, B, nq, nkv, hd, page, window, scale, nsplit, part_o, part_ml)
     f = _fns.get(("attention_kv4", "br_attn_decode_kv4")) or _fn("attention_kv4", "br_attn_decode_kv4", _KV4_DECODE)
-    rc = f(q.data_ptr(), q_stride, out.data_ptr(), slots.data_ptr(), ctx_lens.data_ptr(), block_table.data_ptr(), block_table.size(0),
-           block_table.size(1), cache.data_ptr(), cache.size(0), B, nq, nkv, hd, min(window or 0, 0x7fffffff), scale, nsplit, _ptr(part_o), _ptr(part_ml), _stream())
+    rc = f(q.data_ptr(), q_stride, out.data_ptr(), slots.data_ptr(), ctx_lens.data_ptr(), block_table.data_ptr(), n_slots,
+           table_pages, cache.data_ptr(), pages, B, nq, nkv, hd, min(window or 0, 0x7fffffff), scale, nsplit, _ptr(part_o), _ptr(part_ml), _stream())
     if rc:
         _check(rc, name)
 
@@ -2079,15 +2090,15 @@ def attention_prefill_kv4(q: torch.Tensor, q_stride: int, out: torch.Tensor, cu_
     name = "attention_prefill_kv4"
     _kv4_here(name, out, cu_seqlens, slots, ctx_lens, block_table, cache, part_o, part_ml)
     _kv4_q_here(name, q, out)
-    T = out.size(0)
-    _attention_kv4(name, q, q_stride, out, slots, ctx_lens, block_table, cache, B, T, nq, nkv, hd, page, window, scale, nsplit, part_o, part_ml)
+    T = out.shape[0] if out.dim() == 2 else 0
+    pages, n_slots, table_pages = _attention_kv4(name, q, q_stride, out, slots, ctx_lens, block_table, cache, B, T, nq, nkv, hd, page, window, scale, nsplit, part_o, part_ml)
     if cu_seqlens.dtype is not torch.int32 or cu_seqlens.numel() < B + 1:
         _kv4_fail(name, "cu_seqlens int32 [B + 1]")
     if not 0 <= max_new <= T:
         _kv4_fail(name, f"max_new {max_new} of {T} rows")
     f = _fns.get(("attention_kv4", "br_attn_prefill_kv4")) or _fn("attention_kv4", "br_attn_prefill_kv4", _KV4_PREFILL)
     rc = f(q.data_ptr(), q_stride, out.data_ptr(), cu_seqlens.data_ptr(), slots.data_ptr(), ctx_lens.data_ptr(), block_table.data_ptr(),
-           block_table.size(0), block_table.size(1), cache.data_ptr(), cache.size(0), B, max_new, T, nq, nkv, hd, min(window or 0, 0x7fffffff), scale, nsplit,
+           n_slots, table_pages, cache.data_ptr(), pages, B, max_new, T, nq, nkv, hd, min(window or 0, 0x7fffffff), scale, nsplit,
            _ptr(part_o), _ptr(part_ml), _stream())
     if rc:
         _check(rc, name)
