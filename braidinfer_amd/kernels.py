@@ -1887,36 +1887,37 @@ def _kv4_fail(name: str, why: str):
 
 
 # These calls take longer on the host than the smallest of them on the GPU: checks ask torch for as little as they can (a shape
-# once, not its sizes; the device's number, which says at once that a tensor is on the GPU and on the current one), and messages are put
-# together only where one is needed (8 rows written and read back: 19.2 us a pass before, 15.5 now; their kernels take 5.3, two launches
-# alone 8.1).
-def _kv4_here(name: str, *tensors) -> None:
-    """Every tensor dense and on the current device, whose stream the kernels are launched on."""
-    if not tensors[0].is_cuda:
-        raise KernelError(f"{name}: tensor on {tensors[0].device}; kernels run on the GPU only")
-    here = _current_device()
+# once, not its sizes; the device's number, which says at once that a tensor is on the GPU and on the current one; all in a
+# condition), and who is wrong is found out only where one is (8 rows written and read back: 19.2 us a pass before, 14.2 now; their kernels
+# take 5.3, two launches alone 8.1).
+_kv4_device = _current_device or torch.cuda.current_device
+
+
+def _kv4_elsewhere(name: str, *tensors) -> None:
+    """Raises for the tensor that is not dense or not on the current device, whose stream the kernels are launched on."""
     for t in tensors:
         if t is None:
             continue
-        if t.get_device() != here:
-            if not t.is_cuda:
-                raise KernelError(f"{name}: tensor on {t.device}; kernels run on the GPU only")
-            raise KernelError(f"{name}: tensor on {t.device}, the current device is cuda:{here}")
+        if not t.is_cuda:
+            _kv4_fail(name, f"tensor on {t.device}; kernels run on the GPU only")
+        if t.get_device() != _kv4_device():
+            _kv4_fail(name, f"tensor on {t.device}, the current device is cuda:{_kv4_device()}")
         if not t.is_contiguous():
-            raise KernelError(f"{name}: tensor of shape {tuple(t.shape)} is not contiguous")
+            _kv4_fail(name, f"tensor of shape {tuple(t.shape)} is not contiguous")
 
 
-def _kv4_cache(name: str, cache: torch.Tensor, block_table: torch.Tensor, nkv: int, hd: int, page: int):
-    """The pages of the cache, the rows and columns of the table."""
+def _kv4_cache(name: str, cache: torch.Tensor, at: int, nkv: int, hd: int, page: int) -> int:
+    """The pages of the cache at address `at`."""
     if page != KV4_PAGE:
         _kv4_fail(name, f"pages of {KV4_PAGE} tokens")
     shape = cache.shape
-    if not (nkv > 0 and cache.dtype is torch.uint8 and len(shape) == 3 and shape[1:] == (nkv, kv4_head_bytes(hd)) and cache.data_ptr() % 16 == 0):
+    if cache.dtype is not torch.uint8 or len(shape) != 3 or nkv < 1 or shape[1] != nkv or shape[2] != kv4_head_bytes(hd) or at % 16:
         _kv4_fail(name, f"cache unit must be uint8 [pages, nkv, {kv4_head_bytes(hd)}], 16-byte aligned")
-    return (shape[0], *_kv4_table(name, block_table))
+    return shape[0]
 
 
 def _kv4_table(name: str, block_table: torch.Tensor):
+    """Its rows and columns."""
     shape = block_table.shape
     if len(shape) != 2 or block_table.dtype is not torch.int32:
         _kv4_fail(name, "block table int32 [slots, pages]")
@@ -1924,7 +1925,8 @@ def _kv4_table(name: str, block_table: torch.Tensor):
 
 
 def _kv4_rows(name: str, positions, seq_of_token, slots, T: int) -> None:
-    if not (positions.dtype is torch.int32 and seq_of_token.dtype is torch.int32 and slots.dtype is torch.int32):
+    i32 = torch.int32
+    if positions.dtype is not i32 or seq_of_token.dtype is not i32 or slots.dtype is not i32:
         _kv4_fail(name, "positions, seq_of_token and slots must be int32")
     if positions.numel() < T or seq_of_token.numel() < T:
         _kv4_fail(name, "positions shorter than tokens")
@@ -1936,6 +1938,14 @@ _KV4_DECODE = [_P, c_size_t, _P, _P, _P, _P, c_int, c_int, _P] + [c_int] * 6 + [
 _KV4_PREFILL = [_P, c_size_t, _P, _P, _P, _P, _P, c_int, c_int, _P] + [c_int] * 8 + [c_float, c_int, _P, _P, _P]
 
 
+_kv4_fns = {}    # entry point -> the C function
+
+
+def _kv4_fn(module: str, name: str, argtypes):
+    _kv4_fns[name] = f = _fn(module, name, argtypes)
+    return f
+
+
 def rope_kv4_write(qkv: torch.Tensor, cos: Optional[torch.Tensor], sin: Optional[torch.Tensor], positions: torch.Tensor,
                    seq_of_token: torch.Tensor, slots: torch.Tensor, block_table: torch.Tensor, cache: Optional[torch.Tensor],
                    nq: int, nkv: int, hd: int, rotary_dim: int, adjacent: bool, page: int, write_cache: bool) -> None:
@@ -1943,7 +1953,10 @@ def rope_kv4_write(qkv: torch.Tensor, cos: Optional[torch.Tensor], sin: Optional
     place, and puts rotated keys (rounded to the rows' type first) and values into their pages.  No two tokens of a step may
     stand at the same place of one slot."""
     name = "rope_kv4_write"
-    _kv4_here(name, qkv, positions, seq_of_token, slots, block_table, cos, sin, cache)
+    if not (qkv.is_cuda and _kv4_device() == qkv.get_device() == positions.get_device() == seq_of_token.get_device() == slots.get_device()
+            == block_table.get_device() and qkv.is_contiguous() and positions.is_contiguous() and seq_of_token.is_contiguous()
+            and slots.is_contiguous() and block_table.is_contiguous()):
+        _kv4_elsewhere(name, qkv, positions, seq_of_token, slots, block_table)
     shape = qkv.shape
     if len(shape) != 2 or nq < 0 or shape[1] != (nq + 2 * nkv) * hd:
         _kv4_fail(name, "qkv width is not (nq + 2 nkv) * head_dim")
@@ -1956,20 +1969,24 @@ def rope_kv4_write(qkv: torch.Tensor, cos: Optional[torch.Tensor], sin: Optional
     if (cos is None) != (sin is None):
         _kv4_fail(name, "both rotary tables, or none")
     if cos is not None:
+        _kv4_elsewhere(name, cos, sin)
         if not 0 <= rotary_dim <= hd or rotary_dim % 2:
             _kv4_fail(name, f"rotary_dim {rotary_dim} must be even, at most {hd}")
         if not (cos.dtype is torch.float32 and sin.dtype is torch.float32 and min(cos.numel(), sin.numel()) >= T * (rotary_dim // 2)
                 and cos.data_ptr() % 16 == 0 and sin.data_ptr() % 16 == 0):
             _kv4_fail(name, "rotary tables must be float32 [T, rotary_dim / 2], 16-byte aligned")
+    n_slots, table_pages = _kv4_table(name, block_table)
+    pages = cache_at = 0
     if write_cache:
         if cache is None:
             _kv4_fail(name, "no cache to write to")
-        pages, n_slots, table_pages = _kv4_cache(name, cache, block_table, nkv, hd, page)
-    else:
-        pages, (n_slots, table_pages) = 0, _kv4_table(name, block_table)
-    f = _fns.get(("kv4_cache", "br_rope_kv4_write")) or _fn("kv4_cache", "br_rope_kv4_write", _KV4_WRITE)
+        if cache.get_device() != qkv.get_device() or not cache.is_contiguous():
+            _kv4_elsewhere(name, cache)
+        cache_at = cache.data_ptr()
+        pages = _kv4_cache(name, cache, cache_at, nkv, hd, page)
+    f = _kv4_fns.get("br_rope_kv4_write") or _kv4_fn("kv4_cache", "br_rope_kv4_write", _KV4_WRITE)
     rc = f(at, _is_bf16(qkv, name), _ptr(cos), _ptr(sin), positions.data_ptr(), seq_of_token.data_ptr(), slots.data_ptr(), slots.numel(),
-           block_table.data_ptr(), n_slots, table_pages, _ptr(cache), pages, T, nq, nkv, hd,
+           block_table.data_ptr(), n_slots, table_pages, cache_at, pages, T, nq, nkv, hd,
            rotary_dim if cos is not None else 0, int(adjacent), int(write_cache), _stream())
     if rc:
         _check(rc, name)
@@ -1980,7 +1997,11 @@ def kv4_read(k_out: torch.Tensor, v_out: torch.Tensor, positions: torch.Tensor, 
     """k_out[t], v_out[t] [T, nkv * hd] = what the cache holds for position positions[t] of sequence seq_of_token[t], exactly
     (bfloat16 or float32).  Rows of padding sequences (slot -1) are left as they are."""
     name = "kv4_read"
-    _kv4_here(name, k_out, v_out, positions, seq_of_token, slots, block_table, cache)
+    if not (k_out.is_cuda and _kv4_device() == k_out.get_device() == v_out.get_device() == positions.get_device() == seq_of_token.get_device()
+            == slots.get_device() == block_table.get_device() == cache.get_device() and k_out.is_contiguous() and v_out.is_contiguous()
+            and positions.is_contiguous() and seq_of_token.is_contiguous() and slots.is_contiguous() and block_table.is_contiguous()
+            and cache.is_contiguous()):
+        _kv4_elsewhere(name, k_out, v_out, positions, seq_of_token, slots, block_table, cache)
     shape = k_out.shape
     if len(shape) != 2 or shape != v_out.shape or shape[1] != nkv * hd or k_out.dtype is not v_out.dtype:
         _kv4_fail(name, "k_out and v_out must be [T, nkv * hd] of one type")
@@ -1989,10 +2010,12 @@ def kv4_read(k_out: torch.Tensor, v_out: torch.Tensor, positions: torch.Tensor, 
     if k_at % 16 or v_at % 16:
         _kv4_fail(name, "rows must be 16-byte aligned")
     _kv4_rows(name, positions, seq_of_token, slots, T)
-    pages, n_slots, table_pages = _kv4_cache(name, cache, block_table, nkv, hd, page)
-    f = _fns.get(("kv4_cache", "br_kv4_read")) or _fn("kv4_cache", "br_kv4_read", _KV4_READ)
+    cache_at = cache.data_ptr()
+    pages = _kv4_cache(name, cache, cache_at, nkv, hd, page)
+    n_slots, table_pages = _kv4_table(name, block_table)
+    f = _kv4_fns.get("br_kv4_read") or _kv4_fn("kv4_cache", "br_kv4_read", _KV4_READ)
     rc = f(k_at, v_at, _is_bf16(k_out, name), positions.data_ptr(), seq_of_token.data_ptr(), slots.data_ptr(), slots.numel(),
-           block_table.data_ptr(), n_slots, table_pages, cache.data_ptr(), pages, T, nkv, hd, _stream())
+           block_table.data_ptr(), n_slots, table_pages, cache_at, pages, T, nkv, hd, _stream())
     if rc:
         _check(rc, name)
 
@@ -2025,40 +2048,44 @@ def attention_kv4_splits(n_seqs: int, max_new: int, nq: int, nkv: int, hd: int, 
 
 
 def _attention_kv4(name, q, q_stride, out, slots, ctx_lens, block_table, cache, B, T, nq, nkv, hd, page, window, scale, nsplit, part_o, part_ml):
-    """The pages of the cache, the rows and columns of the table."""
-    bf16 = torch.bfloat16
+    """The arguments of both entry points from the queries' address on to the cache's pages are sound; the addresses and sizes among
+    them that torch has been asked for."""
+    # queries may be columns of wider rows
+    if not (out.is_cuda and _kv4_device() == out.get_device() == q.get_device() == slots.get_device() == ctx_lens.get_device()
+            == block_table.get_device() == cache.get_device() and out.is_contiguous() and slots.is_contiguous() and ctx_lens.is_contiguous()
+            and block_table.is_contiguous() and cache.is_contiguous()):
+        _kv4_elsewhere(name, out, slots, ctx_lens, block_table, cache)
+        _kv4_fail(name, f"queries on {q.device}, the output on {out.device}")
+    bf16, i32 = torch.bfloat16, torch.int32
     if q.dtype is not bf16 or out.dtype is not bf16:
         _kv4_fail(name, "bfloat16 only")
-    sizes = _kv4_cache(name, cache, block_table, nkv, hd, page)
-    shape = out.shape
-    if nq <= 0 or nq % nkv or len(shape) != 2 or shape[1] != nq * hd or shape[0] < T:
-        _kv4_fail(name, "out must be [T, nq * hd]")
-    if not (slots.dtype is torch.int32 and ctx_lens.dtype is torch.int32 and slots.numel() >= B and ctx_lens.numel() >= B):
+    cache_at, out_at, q_at = cache.data_ptr(), out.data_ptr(), q.data_ptr()
+    pages = _kv4_cache(name, cache, cache_at, nkv, hd, page)
+    width, shape = nq * hd, out.shape
+    if nq <= 0 or nq % nkv or len(shape) != 2 or shape[1] != width or shape[0] < T or out_at % 16:
+        _kv4_fail(name, "out must be [T, nq * hd], 16-byte aligned")
+    if slots.dtype is not i32 or ctx_lens.dtype is not i32 or slots.numel() < B or ctx_lens.numel() < B:
         _kv4_fail(name, "slots and ctx_lens int32 [B]")
     if not scale > 0:
         _kv4_fail(name, f"the score scale must be positive, not {scale} (the kernels take the row maximum before scaling)")
     if window is not None and window <= 0:
         _kv4_fail(name, f"the window must be positive or None, not {window}")
+    o_at = ml_at = 0
     if nsplit != 1:
         if not 1 <= nsplit <= 64:
             _kv4_fail(name, f"1 to 64 runs, not {nsplit}")
+        _kv4_elsewhere(name, part_o, part_ml)
         if not (part_o is not None and part_ml is not None and part_o.dtype is torch.float32 and part_ml.dtype is torch.float32
-                and part_o.numel() >= T * nq * nsplit * hd and part_ml.numel() >= T * nq * nsplit * 2 and part_o.data_ptr() % 16 == 0):
+                and part_o.numel() >= T * width * nsplit and part_ml.numel() >= T * nq * nsplit * 2 and part_o.data_ptr() % 16 == 0):
             _kv4_fail(name, "scratch for the runs is too small")
+        o_at, ml_at = part_o.data_ptr(), part_ml.data_ptr()
     # q's storage holds T rows of nq * hd elements, q_stride apart, from its first element on
-    width = nq * hd
-    if q_stride < width or q_stride % 8 or q.data_ptr() % 16:
+    if q_stride < width or q_stride % 8 or q_at % 16:
         _kv4_fail(name, "query rows must be 16-byte aligned")
     rows = (T - 1) * q_stride + width
     if T > 0 and rows > q.numel() and rows > q.untyped_storage().nbytes() // 2 - q.storage_offset():
         _kv4_fail(name, f"q holds fewer than {T} rows of {width}, {q_stride} apart")
-    return sizes
-
-
-def _kv4_q_here(name: str, q: torch.Tensor, out: torch.Tensor) -> None:
-    """Queries may be columns of wider rows: on the device of the others, dense or not."""
-    if q.get_device() != out.get_device():
-        _kv4_fail(name, f"queries on {q.device}, the output on {out.device}")
+    return q_at, out_at, (block_table.data_ptr(), *_kv4_table(name, block_table), cache_at, pages), o_at, ml_at
 
 
 def attention_decode_kv4(q: torch.Tensor, q_stride: int, out: torch.Tensor, slots: torch.Tensor, ctx_lens: torch.Tensor,
@@ -2069,12 +2096,11 @@ def attention_decode_kv4(q: torch.Tensor, q_stride: int, out: torch.Tensor, slot
     already (`rope_kv4_write`).  Rows of padding sequences, and of sequences of no tokens, are zero.  `nsplit`:
     `attention_kv4_splits`.  Two calls that may run at the same time need scratch of their own."""
     name = "attention_decode_kv4"
-    _kv4_here(name, out, slots, ctx_lens, block_table, cache, part_o, part_ml)
-    _kv4_q_here(name, q, out)
-    pages, n_slots, table_pages = _attention_kv4(name, q, q_stride, out, slots, ctx_lens, block_table, cache, B, B, nq, nkv, hd, page, window, scale, nsplit, part_o, part_ml)
-    f = _fns.get(("attention_kv4", "br_attn_decode_kv4")) or _fn("attention_kv4", "br_attn_decode_kv4", _KV4_DECODE)
-    rc = f(q.data_ptr(), q_stride, out.data_ptr(), slots.data_ptr(), ctx_lens.data_ptr(), block_table.data_ptr(), n_slots,
-           table_pages, cache.data_ptr(), pages, B, nq, nkv, hd, min(window or 0, 0x7fffffff), scale, nsplit, _ptr(part_o), _ptr(part_ml), _stream())
+    q_at, out_at, held, o_at, ml_at = _attention_kv4(name, q, q_stride, out, slots, ctx_lens, block_table, cache, B, B, nq, nkv, hd, page, window,
+                                                     scale, nsplit, part_o, part_ml)
+    f = _kv4_fns.get("br_attn_decode_kv4") or _kv4_fn("attention_kv4", "br_attn_decode_kv4", _KV4_DECODE)
+    rc = f(q_at, q_stride, out_at, slots.data_ptr(), ctx_lens.data_ptr(), *held, B, nq, nkv, hd, min(window or 0, 0x7fffffff), scale, nsplit,
+           o_at, ml_at, _stream())
     if rc:
         _check(rc, name)
 
@@ -2088,18 +2114,18 @@ def attention_prefill_kv4(q: torch.Tensor, q_stride: int, out: torch.Tensor, cu_
     the most of one sequence.  Rows of padding sequences are zero, rows behind the last sequence stay as they are.  `nsplit`:
     `attention_kv4_splits`.  Two calls that may run at the same time need scratch of their own."""
     name = "attention_prefill_kv4"
-    _kv4_here(name, out, cu_seqlens, slots, ctx_lens, block_table, cache, part_o, part_ml)
-    _kv4_q_here(name, q, out)
     T = out.shape[0] if out.dim() == 2 else 0
-    pages, n_slots, table_pages = _attention_kv4(name, q, q_stride, out, slots, ctx_lens, block_table, cache, B, T, nq, nkv, hd, page, window, scale, nsplit, part_o, part_ml)
+    q_at, out_at, held, o_at, ml_at = _attention_kv4(name, q, q_stride, out, slots, ctx_lens, block_table, cache, B, T, nq, nkv, hd, page, window,
+                                                     scale, nsplit, part_o, part_ml)
+    if cu_seqlens.get_device() != out.get_device() or not cu_seqlens.is_contiguous():
+        _kv4_elsewhere(name, cu_seqlens)
     if cu_seqlens.dtype is not torch.int32 or cu_seqlens.numel() < B + 1:
         _kv4_fail(name, "cu_seqlens int32 [B + 1]")
     if not 0 <= max_new <= T:
         _kv4_fail(name, f"max_new {max_new} of {T} rows")
-    f = _fns.get(("attention_kv4", "br_attn_prefill_kv4")) or _fn("attention_kv4", "br_attn_prefill_kv4", _KV4_PREFILL)
-    rc = f(q.data_ptr(), q_stride, out.data_ptr(), cu_seqlens.data_ptr(), slots.data_ptr(), ctx_lens.data_ptr(), block_table.data_ptr(),
-           n_slots, table_pages, cache.data_ptr(), pages, B, max_new, T, nq, nkv, hd, min(window or 0, 0x7fffffff), scale, nsplit,
-           _ptr(part_o), _ptr(part_ml), _stream())
+    f = _kv4_fns.get("br_attn_prefill_kv4") or _kv4_fn("attention_kv4", "br_attn_prefill_kv4", _KV4_PREFILL)
+    rc = f(q_at, q_stride, out_at, cu_seqlens.data_ptr(), slots.data_ptr(), ctx_lens.data_ptr(), *held, B, max_new, T, nq, nkv, hd,
+           min(window or 0, 0x7fffffff), scale, nsplit, o_at, ml_at, _stream())
     if rc:
         _check(rc, name)
 

@@ -221,3 +221,38 @@ def test_lists_longer_than_the_kernel_counts_are_refused():
     with pytest.raises(KernelError):
         K.attention_decode_kv4(q, 32, out, dev([0] * 40), dev([64] * 40), table, cache, 40, 1, 1, 32, PAGE, None, 0.2, 2, *part)
     assert (out == 1).all()
+
+
+def test_outputs_and_scratch_that_are_not_aligned_or_elsewhere_are_refused():
+    c = Written([70], 1, 64)
+    q = torch.zeros(4, 64, device="cuda").bfloat16()
+    room = torch.ones(4 * 64 + 8, device="cuda").bfloat16()
+    good, odd = room[:256].view(4, 64), room[2:258].view(4, 64)
+    part = [torch.zeros(4 * 2 * x, device="cuda") for x in (64, 2)]
+
+    def one(out, nsplit=1, part_o=None, part_ml=None, slots=dev(c.slots)):
+        K.attention_decode_kv4(q, 64, out, slots, dev([70]), c.table, c.cache, 1, 1, 1, 64, PAGE, None, 0.1, nsplit, part_o, part_ml)
+
+    def many(out, nsplit=1, part_o=None, part_ml=None, cu=dev([0, 4])):
+        K.attention_prefill_kv4(q, 64, out, cu, dev(c.slots), dev([70]), c.table, c.cache, 1, 4, 1, 1, 64, PAGE, None, 0.1, nsplit, part_o, part_ml)
+
+    for call in (one, many):
+        with pytest.raises(KernelError, match="aligned"):
+            call(odd)
+        with pytest.raises(KernelError, match="scratch"):
+            call(good, 2)
+        with pytest.raises(KernelError, match="GPU only"):
+            call(good, 2, part[0].cpu(), part[1])
+        with pytest.raises(KernelError, match="contiguous"):
+            call(good, 2, part[0], torch.zeros(16, 2, device="cuda").t())
+        with pytest.raises(KernelError, match="64 runs"):
+            call(good, 0)
+        with pytest.raises(KernelError, match="GPU only"):
+            call(good.cpu())
+    with pytest.raises(KernelError, match="GPU only"):
+        one(good, slots=dev(c.slots).cpu())
+    with pytest.raises(KernelError, match="GPU only"):
+        many(good, cu=dev([0, 4]).cpu())
+    assert (room == 1).all()
+    one(good, 2, *part)
+    many(good, 2, *part)

@@ -161,3 +161,20 @@ def test_what_the_cache_takes_and_what_is_refused(models):
         B.Engine.from_folder(folder, dtype="float32", kv_cache="mxfp4")
     with pytest.raises(ConfigError):
         B.Engine.from_folder(folder, kv_cache="int4")
+
+
+def test_recorded_steps_over_long_contexts(models, monkeypatch):
+    """Contexts long enough that single tokens go over them in shares of one list, from recorded graphs, beside a short one."""
+    from braidinfer_amd import kernels as K
+    eng, _, cfg, w = models("plain")
+    assert K.attention_kv4_splits(2, 1, 8, 2, 128, 1400) > 1
+    rng = np.random.default_rng(4)
+    lens = [1400, 70]
+    seqs = [[int(t) for t in rng.integers(0, cfg["vocab_size"], n + 8)] for n in lens]
+    slots = [eng.alloc_slot() for _ in lens]
+    got = [eng.step([StepEntry(s, q[:n], [n - 1]) for s, q, n in zip(slots, seqs, lens)]).cpu().numpy()]
+    for i in range(8):
+        got.append(eng.step([StepEntry(s, [q[n + i]], [0]) for s, q, n in zip(slots, seqs, lens)]).cpu().numpy())
+    for b, (s, q, n) in enumerate(zip(slots, seqs, lens)):
+        close([g[b] for g in got], logits_over(eng, s, cfg, w, q, monkeypatch)[n - 1:n + 8])
+        eng.free_slot(s)
