@@ -717,7 +717,7 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(M > 4 ?
     const int c = lane & 31, g = lane >> 5;
     const int last = (int)(rows_total < (long long)(tile + 1) * tile_rows ? rows_total : (long long)(tile + 1) * tile_rows) - 1;       // of the tile's
     const bool wave_ok = row0 <= last, row_ok = row0 + c <= last;
-    const int rr = row_ok ? row0 + c : last;
+    const int rr = row_ok ? row0 + c : last;                                     // lanes behind the last row work on it too and store nothing
     const int tok = rr / G, head = kvh * G + rr % G;
     const size_t orow = (size_t)(t0 + tok) * nq + head;
     const int slot = seqs.slots[b];
@@ -892,12 +892,12 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(M > 4 ?
 #pragma unroll
             for (int k = 0; k < 2 * M; ++k) s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(*(const bf16x8*)(ks + k * 1024), qf[k], s, 0, 0, 0);
             // s[r]: key kb + 16 (r / 8) + 8 g + r % 8, row = this lane's column
-            const bool whole = row0 + 31 <= last && kb + 31 <= pq_min_w && (window <= 0 || kb > pq_max_w - window);
+            const bool whole = kb + 31 <= pq_min_w && (window <= 0 || kb > pq_max_w - window);
             if (!whole) {
 #pragma unroll
                 for (int r = 0; r < 16; ++r) {
                     const int key = kb + 16 * (r >> 3) + 8 * g + (r & 7);
-                    const bool ok = row_ok && key <= pq && (window <= 0 || key > pq - window);
+                    const bool ok = key <= pq && (window <= 0 || key > pq - window);
                     s[r] = ok ? s[r] : -INFINITY;
                 }
             }
