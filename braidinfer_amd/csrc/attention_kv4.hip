@@ -688,7 +688,7 @@ __device__ __forceinline__ int kv4_row_of_key(int u) { return (u & 3) | (((u >> 
 __device__ __forceinline__ int kv4_value_row(int row, int i2) { return row ^ ((row >> 4) | ((i2 & 3) << 1)); }
 
 template <int M, int NW, int KH>
-__global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(M > 4 ? 1 : M <= 2 ? 4 : 2, M <= 2 ? 4 : 2))) void attn_prefill_kv4_kernel(const bf16* __restrict__ q, size_t q_stride, bf16* __restrict__ out,
+__global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(NW == 4 ? 1 : M <= 2 ? 4 : 2, M <= 2 ? 4 : 2))) void attn_prefill_kv4_kernel(const bf16* __restrict__ q, size_t q_stride, bf16* __restrict__ out,
                                                                    const int* __restrict__ cu_seqlens, Kv4Seqs seqs,
                                                                    const unsigned char* __restrict__ cache, int nq, int nkv, int window,
                                                                    float scale, const PrefillOrder order, int n_tokens, int tile_rows, int nsplit,
@@ -1061,7 +1061,10 @@ extern "C" int br_attn_prefill_kv4(const void* q, size_t q_stride, void* out, co
     // In runs: 5 tokens behind 3,800 of 8 users 33 / 40, 16 behind 16,000 23.3 / 24.6, 32 behind 16,352 29.3 / 28.1.
     const int cus = br_device_cus() > 0 ? br_device_cus() : 256, each = hd <= 64 ? 2 : 1;
     const long long filled = ((long long)n_tokens * (nq / nkv) + 255) / 256 * nkv;
-    // larger heads have no registers for 8 waves
+    // Heads beyond 128 have no registers for 256 rows, and from 8 waves of 256 channels 34 spill: two prompts of 158 and 109 tokens of 12 heads
+    // over 4 and 24 over 8 take 4 waves of 32 rows, each alone on its SIMD, 19.0 and 19.4 us, 8 waves 19.8 and 22.3; 1,646 tokens 66 / 60, 8,192 947 / 749 (of
+    // heads of 160 740 / 459).
+    const bool half = hd < 256 || nsplit > 1 || max_new > 256;
     const bool wide = hd <= 128 && (nsplit > 1 ? rows > 64 : filled > (each == 2 || B == 1 ? each * cus : cus / 2));
     const int most = wide ? 256 : 128;
     const long long tiles = (rows + most - 1) / most;
@@ -1074,17 +1077,20 @@ extern "C" int br_attn_prefill_kv4(const void* q, size_t q_stride, void* out, co
         if (tiles * nsplit > 0x7fffffffLL) return BR_BAD_ARG;
         grid = dim3((unsigned)(tiles * nsplit), nkv, B);
     } else if (!prefill_order(order, grid, wide ? (rows + 1) / 2 : rows, nkv, B, cus, each)) return BR_BAD_ARG;   // it counts in tiles of 128
-    const size_t lds = 2 * (size_t)2 * KV4_PAGE * hd * 2 + (!wide && hd <= 128 ? 4 * 128 * sizeof(float) : 16 + 2 * (hd / 32) * 8);
+    const size_t lds = 2 * (size_t)2 * KV4_PAGE * hd * 2 + (!wide && half ? 4 * 128 * sizeof(float) : 16 + 2 * (hd / 32) * 8);
     const Kv4Seqs seqs = {slots, ctx_lens, table, n_slots, table_pages, n_pages};
 #define GO(M_, NW_, KH_) { \
         static unsigned long long told; \
         if (lds > 65536 && !kv4_allow((const void*)attn_prefill_kv4_kernel<M_, NW_, KH_>, lds, told)) return BR_LAUNCH_FAILED; \
         attn_prefill_kv4_kernel<M_, NW_, KH_><<<grid, NW_ * 64, lds, s>>>((const bf16*)q, q_stride, (bf16*)out, cu_seqlens, seqs, (const unsigned char*)cache, nq, nkv, window, scale, order, n_tokens, tile_rows, nsplit, part_o, part_ml); }
-#define CASE(M_) case M_: GO(M_, 4, 1) break;
 #define BOTH(M_) case M_: if (wide) GO(M_, 8, 1) else GO(M_, 8, 2) break;
-    switch (hd / 32) { BOTH(1) BOTH(2) BOTH(3) BOTH(4) CASE(5) CASE(6) CASE(7) CASE(8) }
+#define HALF(M_) case M_: GO(M_, 8, 2) break;
+    switch (hd / 32) {
+        BOTH(1) BOTH(2) BOTH(3) BOTH(4) HALF(5) HALF(6) HALF(7)
+        case 8: if (half) GO(8, 8, 2) else GO(8, 4, 1) break;
+    }
+#undef HALF
 #undef BOTH
-#undef CASE
 #undef GO
     const int rc = br_check_launch();
     return rc != BR_OK || nsplit == 1 ? rc : kv4_join<false>(part_o, part_ml, out, n_tokens, nq, hd, nsplit, cu_seqlens + B, seqs, Kv4Runs{}, 1, 1, s);
