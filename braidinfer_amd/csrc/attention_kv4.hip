@@ -415,13 +415,13 @@ struct Kv4State {
             }
         }
     }
-    // the channel of o[tile]'s row r (0..15); SPLIT: the even copy's, the odd one's is the next
-    static __device__ __forceinline__ int channel(int tile, int r) {
-        constexpr int PER = MP >= 4 ? 8 : MP == 2 ? 4 : 2;              // channels of a row in one set
-        const int i = SPLIT ? 2 * tile : tile, in = i % PER;
-        if constexpr (MP >= 4) return 8 * (r + 16 * (i / PER)) + in;
-        else if constexpr (MP == 2) return 8 * (r & 7) + 4 * (r >> 3) + in;
-        else return 8 * (r & 3) + 2 * (r >> 2) + in;
+    // Row r (0..15) of the accumulators of one set is PER neighbouring channels from `channel` on: number e of them in tile set PER + e, or, SPLIT,
+    // in tile (set PER + e) / 2 of copy e % 2.
+    static constexpr int PER = MP >= 4 ? 8 : MP == 2 ? 4 : 2, SETS = 2 * MP / PER;
+    static __device__ __forceinline__ int channel(int set, int r) {
+        if constexpr (MP >= 4) return 8 * (r + 16 * set);
+        else if constexpr (MP == 2) return 8 * (r & 7) + 4 * (r >> 3);
+        else return 8 * (r & 3) + 2 * (r >> 2);
     }
 };
 
@@ -437,9 +437,9 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(M <= 4 && G
     int nq, int nkv, float scale, float* __restrict__ part_o, float* __restrict__ part_ml) {
     typedef Kv4State<M, GB> State;
     typedef kv4_layout<M> L;
-    constexpr int HD = 32 * M, MP = State::MP;
-    constexpr int WSTRIDE = GB * HD + 2 * GB;
-    extern __shared__ float lds[];                      // per wave [GB heads][HD] O, then [GB] m, [GB] l
+    constexpr int HD = 32 * M, MP = State::MP, PER = State::PER;
+    constexpr int OS = State::TILES * 256, WSTRIDE = OS + 2 * GB;
+    extern __shared__ float lds[];                      // per wave its accumulators register by register, [TILES][4][64 lanes], then [GB] m, [GB] l
     const int G = nq / nkv, nhb = (G + GB - 1) / GB;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const Kv4Lane<M> at(lane);
@@ -561,37 +561,50 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(M <= 4 && G
             if (part) v1.template load<1>(part, at);
         }
         st.l = State::sum(st.l);
+        // Register by register no two lanes meet in a bank, neither here nor where they are read (16 heads of 256, head by head and channel by
+        // channel: all 64 lanes in one, 7 us a stretch).
         float* my = lds + wave * WSTRIDE;
-        const int copy = c / GB, h = c % GB;
-        if (copy < (State::SPLIT ? 2 : 1)) {
+        const int copy = c / GB;
 #pragma unroll
-            for (int i = 0; i < State::TILES; ++i)
+        for (int i = 0; i < State::TILES; ++i)
 #pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    const int d = State::channel(i, 4 * g + r) + copy;
-                    if (M == MP || d < HD) my[h * HD + d] = st.o[i][r];
-                }
-        }
-        if (g == 0 && copy == 0) { my[GB * HD + h] = st.m; my[GB * HD + GB + h] = st.l; }
+            for (int r = 0; r < 4; ++r) my[(4 * i + r) * 64 + lane] = st.o[i][r];
+        if (g == 0 && copy == 0) { my[OS + c] = st.m; my[OS + GB + c] = st.l; }
         __syncthreads();
-        for (int i = threadIdx.x; i < nheads * HD; i += 256) {
-            const int hh = i / HD, d = i % HD;
+        for (int u = threadIdx.x; u < GB * 16 * State::SETS; u += 256) {
+            const int h = u % GB, ug = u / GB & 3, ur = u / (4 * GB) & 3, set = u / (16 * GB), d = State::channel(set, 4 * ug + ur);
+            if (h >= nheads || (M != MP && d >= HD)) continue;
             float mx = -INFINITY;
 #pragma unroll
-            for (int w = 0; w < 4; ++w) mx = fmaxf(mx, lds[w * WSTRIDE + GB * HD + hh]);
+            for (int w = 0; w < 4; ++w) mx = fmaxf(mx, lds[w * WSTRIDE + OS + h]);
             const float use = mx == -INFINITY ? 0.f : mx;
-            float sum = 0.f, o = 0.f;
+            float sum = 0.f, v[PER];
+#pragma unroll
+            for (int e = 0; e < PER; ++e) v[e] = 0.f;
 #pragma unroll
             for (int w = 0; w < 4; ++w) {
-                const float f = kv4_exp2(lds[w * WSTRIDE + GB * HD + hh] - use);
-                sum += lds[w * WSTRIDE + GB * HD + GB + hh] * f;
-                o += lds[w * WSTRIDE + hh * HD + d] * f;
+                const float f = kv4_exp2(lds[w * WSTRIDE + OS + h] - use);
+                sum += lds[w * WSTRIDE + OS + GB + h] * f;
+#pragma unroll
+                for (int e = 0; e < PER; ++e) {
+                    const int tile = State::SPLIT ? (set * PER + e) / 2 : set * PER + e;
+                    v[e] += lds[w * WSTRIDE + (4 * tile + ur) * 64 + 16 * ug + (State::SPLIT ? (e & 1) * GB : 0) + h] * f;
+                }
             }
-            const size_t row = (size_t)now.b * nq + head0 + hh;
-            if (now.whole) out[row * HD + d] = (bf16)(sum == 0.f ? 0.f : o / sum);
-            else {
+            const size_t row = (size_t)now.b * nq + head0 + h;
+            typedef float vf __attribute__((ext_vector_type(PER)));
+            typedef bf16 vb __attribute__((ext_vector_type(PER)));
+            if (now.whole) {
+                vb y;
+#pragma unroll
+                for (int e = 0; e < PER; ++e) y[e] = (bf16)(sum == 0.f ? 0.f : v[e] / sum);
+                *(vb*)(out + row * HD + d) = y;
+            } else {
                 const size_t i_ = row * runs.nsplit + now.piece;
-                part_o[i_ * HD + d] = o;
+                vf y;
+#pragma unroll
+                for (int e = 0; e < PER; ++e) y[e] = v[e];
+                *(vf*)(part_o + i_ * HD + d) = y;
                 if (d == 0) { part_ml[i_ * 2] = mx; part_ml[i_ * 2 + 1] = sum; }
             }
         }
@@ -1030,7 +1043,8 @@ extern "C" int br_attn_decode_kv4(const void* q, size_t q_stride, void* out, con
     const int wgs = (int)((pages + 3) / 4 < all ? (pages + 3) / 4 > 0 ? (pages + 3) / 4 : 1 : all);
     const Kv4Runs runs = {B, window, groups, wgs, nsplit, (float)(1.00001 * groups / wgs), (float)(1.00001 / (nsplit > 1 ? nsplit - 1 : 1))};
     const dim3 grid = nsplit > 1 ? dim3(wgs) : dim3(groups, B);
-    const size_t lds = 4 * ((size_t)gb * hd + 2 * gb) * sizeof(float);
+    const int mp = hd > 128 ? 8 : hd == 96 ? 4 : hd / 32;                   // Kv4Keys::MP
+    const size_t lds = 4 * ((size_t)(gb < 16 ? mp : 2 * mp) * 256 + 2 * gb) * sizeof(float);
     const Kv4Seqs seqs = {slots, ctx_lens, table, n_slots, table_pages, n_pages};
 #define GO(M_, GB_) { \
         static unsigned long long told; \
