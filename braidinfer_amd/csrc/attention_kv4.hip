@@ -425,6 +425,11 @@ struct Kv4State {
     }
 };
 
+// How many workgroups a compute unit holds: what their registers allow.  With two of 16 heads beyond 128 28 to 37 spill: 64 sequences of 128 to 8,192
+// tokens through 8 kv heads of 256 183 us, so 140; 32 of 2,000 of 160 38.7 and 31.7.  A step's shares are as many as are resident: 3 a unit where 1 is
+// 159, where 2 are (32 heads of 256 over 8, 11 sequences to 6,799; 128 of 128, 16 of 8,000) 37 us against 29 and 44 against 35.
+constexpr int kv4_decode_resident(int hd, int gb) { return hd <= 128 ? (gb < 16 ? 3 : 2) : gb < 16 ? 2 : 1; }
+
 // block = 256: the 4 waves take the pages of a stretch in turn, each with keys and values straight from memory into registers, and are
 // joined in LDS in wave order where the stretch ends; nothing else is shared between them.  A wave's next page, of this stretch or
 // the next, is asked for piece by piece, each as soon as the registers that held the present page's are free.
@@ -432,7 +437,7 @@ struct Kv4State {
 // Bytes bound it where there are many: 16 sequences of 32,768 (8 kv heads of 128) in 93 us, 6.1 TB/s, 64 of 128 to 8,192 in 52 us, 5.6 TB/s; the
 // waits for lengths, table and first page (together 5 us) where there are few: one of 1,088 in 9 us.
 template <int M, int GB>
-__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(M <= 4 && GB < 16 ? 3 : 2, M <= 4 && GB < 16 ? 3 : 2))) void attn_decode_kv4_kernel(
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(kv4_decode_resident(32 * M, GB), kv4_decode_resident(32 * M, GB)))) void attn_decode_kv4_kernel(
     const bf16* __restrict__ q, size_t q_stride, bf16* __restrict__ out, Kv4Seqs seqs, Kv4Runs runs, const unsigned char* __restrict__ cache,
     int nq, int nkv, float scale, float* __restrict__ part_o, float* __restrict__ part_ml) {
     typedef Kv4State<M, GB> State;
@@ -1035,7 +1040,7 @@ extern "C" int br_attn_decode_kv4(const void* q, size_t q_stride, void* out, con
     // heads that share a kv head go as columns of one product: 4, 8 or 16 at a time
     const int G = nq / nkv, gb = G <= 4 ? 4 : G <= 8 ? 8 : 16, groups = nkv * ((G + gb - 1) / gb);
     if ((long long)B * nq > 0x7fffffffLL) return BR_BAD_ARG;
-    const int cus = br_device_cus(), all = (cus > 0 ? cus : 256) * 3;      // what is resident of the kernels for heads of up to 128
+    const int cus = br_device_cus(), all = (cus > 0 ? cus : 256) * kv4_decode_resident(hd, gb);
     const long long seen = window > 0 && (window + 2LL * KV4_PAGE - 2) / KV4_PAGE < table_pages ? (window + 2LL * KV4_PAGE - 2) / KV4_PAGE : table_pages;
     const long long pages = B * seen * groups, places = pages + (long long)B * groups * KV4_SWITCH;        // of the list at most
     if (places > 0x3fffffffLL) return BR_TOO_LARGE;
