@@ -2040,7 +2040,7 @@ def attention_kv4_splits(n_seqs: int, max_new: int, nq: int, nkv: int, hd: int, 
         # the most pieces of a sequence that the scratch holds: eight times its even share, as one that is longer than the others has
         return max(2, min(64, -(-pages // 4) + 1, 2 + 24 * cus // max(1, groups)))
     # Tiles of 256 rows (128 of heads beyond 128): as many runs at most as fill the compute units once (67 tokens behind 16,344: 608 us
-    # whole, 79 in 8 runs, 50 in 16, 73 in 20).  A page takes a run about `page` us, the join 4 and `run` for each run's sums (one kv head, 6
+    # whole, 79 in 8 runs, 50 in 16, 73 in 20).  A page takes a run about `page` us, the join 7 with its launch and `run` for each run's sums (one kv head, 6
     # and 128 tokens behind 2,048, us whole / in 4 / 16 / 32 runs: heads of 128 44 / 18 / 12.7 / 12.9 and 48 / 27 / 19 / 21, of 256 112 / 30 / 20 / 20
     # and 118 / 39 / 28 / 31; a prompt of 1,024 through 8 kv heads 33 whole, 44 in 2).
     rows, tile = max_new * (nq // nkv), 256 if hd <= 128 else 128
@@ -2054,7 +2054,7 @@ def attention_kv4_splits(n_seqs: int, max_new: int, nq: int, nkv: int, hd: int, 
     n = max(2, int(min(most, (pages * page / run) ** 0.5)))
     each = -(-pages // n)
     n = -(-pages // each)
-    return n if each * page + 4 + n * run < pages * (1.5 if hd <= 128 else 2.0) else 1
+    return n if each * page + 7 + n * run < pages * (1.5 if hd <= 128 else 2.0) else 1
 
 
 def _attention_kv4(name, q, q_stride, out, slots, ctx_lens, block_table, cache, B, T, nq, nkv, hd, page, window, scale, nsplit, part_o, part_ml):
