@@ -667,7 +667,7 @@ __global__ __launch_bounds__(256) void attn_kv4_join_kernel(const float* __restr
         for (int j = 0; j < 4; ++j) {
             const int i = i0 + j * many + sub;
             const float w = __shfl(f, i < n_runs ? i : 0, WAVE);
-            if (i < n_runs && w != 0.f) o += w * x[j];         // a run without a token has written no sums
+            if (i < n_runs) o += w * x[j];         // of a weight of 0 as well: its sums are NaN where a value that the row sees is
         }
     }
     if (sub >= many) o = f32x4{0.f, 0.f, 0.f, 0.f};
