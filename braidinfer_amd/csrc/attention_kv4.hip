@@ -622,15 +622,19 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(kv4_decode_
 }
 
 // The runs of a row added in their order: out = sum_i 2^(m_i - M) o_i / sum_i 2^(m_i - M) l_i.  A wave a row (token, head).
-// `last` (null: none): the number of tokens that sequences hold; rows behind them have no runs and stay as they are.
+// `cu` (null: none): the step's B + 1 offsets; rows in front of the first sequence and behind the last have no runs and stay as they are.
 // RUNS: rows of single tokens, in as many pieces each as the list's places say; those of one are there already.
 template <bool RUNS>
 __global__ __launch_bounds__(256) void attn_kv4_join_kernel(const float* __restrict__ part_o, const float* __restrict__ part_ml,
                                                             bf16* __restrict__ out, size_t rows, int nq, int hd, int nsplit,
-                                                            const int* __restrict__ last, Kv4Seqs seqs, Kv4Runs runs, int G, int gb) {
+                                                            const int* __restrict__ cu, int B, Kv4Seqs seqs, Kv4Runs runs, int G, int gb) {
     const size_t row = (size_t)blockIdx.x * 4 + (threadIdx.x >> 6);
     const int lane = threadIdx.x & 63;
-    if (row >= rows || (last && row >= (size_t)(*last > 0 ? *last : 0) * nq)) return;
+    if (row >= rows) return;
+    if (cu) {
+        const long long first = (long long)cu[0] * nq, end = (long long)cu[B] * nq;
+        if ((long long)row < first || (long long)row >= end) return;
+    }
     // runs are at most 64, one a lane; 16 lanes take 64 channels, so that a run's row is hd / 64 groups of them and the others take
     // further runs at the same time.  Everything is asked for before it is known how many runs there are: of the others nothing is used.
     const float m_ = lane < nsplit ? part_ml[(row * nsplit + lane) * 2] : -INFINITY;
@@ -1025,10 +1029,10 @@ static bool kv4_allow(const void* kernel, size_t lds, unsigned long long& told) 
 #define KV4_SIZES(F) F(1) F(2) F(3) F(4) F(5) F(6) F(7) F(8)
 
 template <bool RUNS>
-static int kv4_join(const float* part_o, const float* part_ml, void* out, long long tokens, int nq, int hd, int nsplit, const int* last,
+static int kv4_join(const float* part_o, const float* part_ml, void* out, long long tokens, int nq, int hd, int nsplit, const int* cu, int B,
                     const Kv4Seqs& seqs, const Kv4Runs& runs, int G, int gb, hipStream_t s) {
     const size_t rows = (size_t)tokens * nq;
-    attn_kv4_join_kernel<RUNS><<<(unsigned)((rows + 3) / 4), 256, 0, s>>>(part_o, part_ml, (bf16*)out, rows, nq, hd, nsplit, last, seqs, runs, G, gb);
+    attn_kv4_join_kernel<RUNS><<<(unsigned)((rows + 3) / 4), 256, 0, s>>>(part_o, part_ml, (bf16*)out, rows, nq, hd, nsplit, cu, B, seqs, runs, G, gb);
     return br_check_launch();
 }
 
@@ -1060,7 +1064,7 @@ extern "C" int br_attn_decode_kv4(const void* q, size_t q_stride, void* out, con
 #undef CASE
 #undef GO
     const int rc = br_check_launch();
-    return rc != BR_OK || nsplit == 1 ? rc : kv4_join<true>(part_o, part_ml, out, B, nq, hd, nsplit, nullptr, seqs, runs, G, gb, s);
+    return rc != BR_OK || nsplit == 1 ? rc : kv4_join<true>(part_o, part_ml, out, B, nq, hd, nsplit, nullptr, B, seqs, runs, G, gb, s);
 }
 
 extern "C" int br_attn_prefill_kv4(const void* q, size_t q_stride, void* out, const int* cu_seqlens, const int* slots, const int* ctx_lens,
@@ -1111,5 +1115,5 @@ extern "C" int br_attn_prefill_kv4(const void* q, size_t q_stride, void* out, co
 #undef BOTH
 #undef GO
     const int rc = br_check_launch();
-    return rc != BR_OK || nsplit == 1 ? rc : kv4_join<false>(part_o, part_ml, out, n_tokens, nq, hd, nsplit, cu_seqlens + B, seqs, Kv4Runs{}, 1, 1, s);
+    return rc != BR_OK || nsplit == 1 ? rc : kv4_join<false>(part_o, part_ml, out, n_tokens, nq, hd, nsplit, cu_seqlens, B, seqs, Kv4Runs{}, 1, 1, s);
 }

@@ -2121,8 +2121,8 @@ def attention_prefill_kv4(q: torch.Tensor, q_stride: int, out: torch.Tensor, cu_
                           part_o: Optional[torch.Tensor] = None, part_ml: Optional[torch.Tensor] = None) -> None:
     """`attention_prefill_bf16` over a cache of 4-bit keys and values, which holds the new tokens already (`rope_kv4_write`):
     sequence b's are rows cu_seqlens[b] .. cu_seqlens[b + 1] of `out` and `q`, the last of its ctx_lens[b] tokens; `max_new` is
-    the most of one sequence.  Rows of padding sequences are zero, rows behind the last sequence stay as they are.  `nsplit`:
-    `attention_kv4_splits`.  Two calls that may run at the same time need scratch of their own."""
+    the most of one sequence.  Rows of padding sequences are zero, rows in front of the first sequence and behind the last stay as they
+    are.  `nsplit`: `attention_kv4_splits`.  Two calls that may run at the same time need scratch of their own."""
     name = "attention_prefill_kv4"
     T = out.shape[0] if out.dim() == 2 else 0
     q_at, out_at, held, o_at, ml_at = _attention_kv4(name, q, q_stride, out, slots, ctx_lens, block_table, cache, B, T, nq, nkv, hd, page, window,

@@ -51,3 +51,24 @@ def test_nan_of_a_run_far_below_reaches_the_rows(hd, nq, nsplit):
         want, size, most = P.attention(q, k, v, 0.5, n - count)
         assert np.isnan(want[:, :, -32:]).all() and np.isfinite(want[:, :, :-32]).all()
         check(prefill(c, q, [count], None, 0.5, nsplit), want, size, most, hd, n)
+
+
+@pytest.mark.parametrize("nsplit", [1, 2, 9])
+def test_rows_in_front_of_the_first_sequence_stay(nsplit):
+    nq, nkv, hd, front, counts, behind = 4, 2, 64, 5, [7, 3], 2
+    c = Cache([400, 90], nkv, hd)
+    kv = c.fill()
+    T = front + sum(counts) + behind
+    q = bf16(np.random.default_rng(0).standard_normal((T, nq, hd)))
+    table, cache = c.tensors
+    out = torch.full((T, nq * hd), 9.0, device="cuda", dtype=torch.bfloat16)
+    part = [torch.full((T * nq * nsplit * x,), 3.0, device="cuda") for x in (hd, 2)] if nsplit > 1 else [None, None]
+    rows = torch.from_numpy(q).reshape(T, -1).bfloat16().cuda()
+    K.attention_prefill_kv4(rows, nq * hd, out, step_of(counts, [0, 0])[2] + front, dev(c.slots), dev(c.lens), table, cache, 2, max(counts), nq, nkv,
+                            hd, PAGE, None, 0.1, nsplit, *part)
+    assert (out[:front] == 9).all() and (out[T - behind:] == 9).all()
+    got, at = out.double().cpu().numpy().reshape(T, nq, hd), front
+    for (k, v), n, length in zip(kv, counts, c.lens):
+        want, size, most = P.attention(q[at:at + n].astype(np.float64), k, v, 0.1, length - n)
+        assert (np.abs(got[at:at + n] - want) <= tolerance(want, size, most, hd, length)).all()
+        at += n
