@@ -1932,6 +1932,16 @@ def _kv4_rows(name: str, positions, seq_of_token, slots, T: int) -> None:
         _kv4_fail(name, "positions shorter than tokens")
 
 
+def _kv4_queries(name: str, q: torch.Tensor, q_stride: int, T: int, width: int) -> None:
+    """Raises unless q's storage holds T rows of `width` 2-byte elements, q_stride apart, from its first element on.  Its elements say
+    so themselves only where they lie side by side: an expanded tensor has more of them than memory."""
+    if q_stride < width or q_stride % 8:
+        _kv4_fail(name, "query rows must be 16-byte aligned")
+    rows = (T - 1) * q_stride + width
+    if T > 0 and not (rows <= q.numel() and q.is_contiguous()) and rows > q.untyped_storage().nbytes() // 2 - q.storage_offset():
+        _kv4_fail(name, f"q holds fewer than {T} rows of {width}, {q_stride} apart")
+
+
 _KV4_WRITE = [_P, c_int, _P, _P, _P, _P, _P, c_int, _P, c_int, c_int, _P] + [c_int] * 8 + [_P]
 _KV4_READ = [_P, _P, c_int, _P, _P, _P, c_int, _P, c_int, c_int, _P] + [c_int] * 4 + [_P]
 _KV4_DECODE = [_P, c_size_t, _P, _P, _P, _P, c_int, c_int, _P] + [c_int] * 6 + [c_float, c_int, _P, _P, _P]
@@ -2089,12 +2099,9 @@ def _attention_kv4(name, q, q_stride, out, slots, ctx_lens, block_table, cache, 
                 and part_o.numel() >= T * width * nsplit and part_ml.numel() >= T * nq * nsplit * 2 and part_o.data_ptr() % 16 == 0):
             _kv4_fail(name, "scratch for the runs is too small")
         o_at, ml_at = part_o.data_ptr(), part_ml.data_ptr()
-    # q's storage holds T rows of nq * hd elements, q_stride apart, from its first element on
-    if q_stride < width or q_stride % 8 or q_at % 16:
+    if q_at % 16:
         _kv4_fail(name, "query rows must be 16-byte aligned")
-    rows = (T - 1) * q_stride + width
-    if T > 0 and rows > q.numel() and rows > q.untyped_storage().nbytes() // 2 - q.storage_offset():
-        _kv4_fail(name, f"q holds fewer than {T} rows of {width}, {q_stride} apart")
+    _kv4_queries(name, q, q_stride, T, width)
     return q_at, out_at, (block_table.data_ptr(), *_kv4_table(name, block_table), cache_at, pages), o_at, ml_at
 
 
