@@ -2086,8 +2086,9 @@ def _attention_kv4(name, q, q_stride, out, slots, ctx_lens, block_table, cache, 
         _kv4_fail(name, "out must be [T, nq * hd], 16-byte aligned")
     if slots.dtype is not i32 or ctx_lens.dtype is not i32 or slots.numel() < B or ctx_lens.numel() < B:
         _kv4_fail(name, "slots and ctx_lens int32 [B]")
-    if not scale > 0:
-        _kv4_fail(name, f"the score scale must be positive, not {scale} (the kernels take the row maximum before scaling)")
+    # positive: the kernels take the row maximum before scaling.  In float, and times log2 e: 0 or infinity times a masked score is NaN.
+    if not 1e-45 <= scale <= 2.3e38:
+        _kv4_fail(name, f"the score scale must be positive and a 32-bit number, not {scale}")
     if window is not None and window <= 0:
         _kv4_fail(name, f"the window must be positive or None, not {window}")
     o_at = ml_at = 0
