@@ -2030,14 +2030,16 @@ def kv4_read(k_out: torch.Tensor, v_out: torch.Tensor, positions: torch.Tensor, 
         _check(rc, name)
 
 
-def attention_kv4_splits(n_seqs: int, max_new: int, nq: int, nkv: int, hd: int, max_ctx: int, window: Optional[int] = None) -> int:
+def attention_kv4_splits(n_seqs: int, max_new: int, nq: int, nkv: int, hd: int, max_ctx: int, window: Optional[int] = None,
+                         decode: Optional[bool] = None) -> int:
     """Into how many runs the 4-bit attention kernels cut the pages that a row sees (1: none), by the step's shape: sequences,
     most new tokens of one, an upper bound of the contexts.  With n > 1 they take scratch part_o of T * nq * n * hd and part_ml of
-    T * nq * n * 2 floats, T the step's tokens."""
+    T * nq * n * 2 floats, T the step's tokens.  `decode`: which of them, `attention_decode_kv4` (True) or `attention_prefill_kv4`
+    (False); None: the former where `max_new` is 1."""
     cus = device_cus()
     seen = max_ctx if window is None else min(max_ctx, window + max_new)
     pages = max(1, -(-seen // KV4_PAGE) + (window is not None))
-    if max_new == 1:
+    if decode if decode is not None else max_new == 1:
         # One workgroup for a sequence and kv head takes 5 us and 0.4 for each page; cut into equal shares of all pages with a second
         # launch that joins them, 11 us and the time of all bytes (8 kv heads of 128, both ways, us: one sequence of 700 tokens 8.3 / 12.3,
         # 1,500 11.5 / 10.2; 8 of 128 to 2,048 15.9 / 13.6; 24 of 1,500 13.9 / 17.8; 32 of 128 to 8,192 52 / 38; 64 of 128 to 2,048 19.5 / 27.4,
@@ -2049,6 +2051,8 @@ def attention_kv4_splits(n_seqs: int, max_new: int, nq: int, nkv: int, hd: int, 
             return 1
         # the most pieces of a sequence that the scratch holds: eight times its even share, as one that is longer than the others has
         return max(2, min(64, -(-pages // 4) + 1, 2 + 24 * cus // max(1, groups)))
+    # (The number above only bounds a sequence's pieces; here every row comes in as many.  One new token each behind 8 of 32,768 by this rule: 4 runs 151
+    # us, where 64 are 221; four of 8,000, 4 kv heads of 64: 16 runs 19.3, 33 26.6.)
     # Tiles of 256 rows (128 of heads beyond 128): as many runs at most as fill the compute units once (67 tokens behind 16,344: 608 us
     # whole, 79 in 8 runs, 50 in 16, 73 in 20).  A page takes a run about `page` us, the join 7 with its launch and `run` for each run's sums (one kv head, 6
     # and 128 tokens behind 2,048, us whole / in 4 / 16 / 32 runs: heads of 128 44 / 18 / 12.7 / 12.9 and 48 / 27 / 19 / 21, of 256 112 / 30 / 20 / 20

@@ -176,7 +176,7 @@ class GQAAttention(Mixer):
         nq, nkv, hd = self.nq, self.nkv, self.hd
         if self.kv_cache is not None:
             B, new = step.n_seqs, 1 if step.is_decode else step.max_new
-            nsplit = K.attention_kv4_splits(B, new, nq, nkv, hd, step.max_ctx_bound, self.window)
+            nsplit = K.attention_kv4_splits(B, new, nq, nkv, hd, step.max_ctx_bound, self.window, step.is_decode)
             part_o = part_ml = None
             if nsplit > 1:
                 part_o = step.ws.get("attn_part_o", (T * nq * nsplit * hd,), torch.float32)
