@@ -256,7 +256,8 @@ def prepare(case, seed):
         state["out"] = torch.zeros((T, nq * hd), dtype=dt, device=dev)
         if own:
             from braidinfer_amd import kernels as K
-            state["nsplit"] = K.attention_kv4_splits(state["B"], max(counts), nq, nkv, hd, max(lens), case["window"] or None)
+            state["nsplit"] = K.attention_kv4_splits(state["B"], max(counts), nq, nkv, hd, max(lens), case["window"] or None,
+                                                     case["task"] == "decode")
             n = state["nsplit"]
             state["part_o"] = torch.empty(T * nq * n * hd, device=dev) if n > 1 else None
             state["part_ml"] = torch.empty(T * nq * n * 2, device=dev) if n > 1 else None
