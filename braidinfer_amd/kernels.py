@@ -1919,8 +1919,8 @@ def _kv4_cache(name: str, cache: torch.Tensor, at: int, nkv: int, hd: int, page:
 def _kv4_table(name: str, block_table: torch.Tensor):
     """Its rows and columns."""
     shape = block_table.shape
-    if len(shape) != 2 or block_table.dtype is not torch.int32:
-        _kv4_fail(name, "block table int32 [slots, pages]")
+    if len(shape) != 2 or block_table.dtype is not torch.int32 or shape[0] > 0x7fffffff or shape[1] > 0x7fffffff:
+        _kv4_fail(name, "block table int32 [slots, pages], each below 2^31")
     return shape
 
 
@@ -1930,6 +1930,8 @@ def _kv4_rows(name: str, positions, seq_of_token, slots, T: int) -> None:
         _kv4_fail(name, "positions, seq_of_token and slots must be int32")
     if positions.numel() < T or seq_of_token.numel() < T:
         _kv4_fail(name, "positions shorter than tokens")
+    if slots.numel() > 0x7fffffff:
+        _kv4_fail(name, "slots of 2^31 sequences and more")
 
 
 def _kv4_queries(name: str, q: torch.Tensor, q_stride: int, T: int, width: int) -> None:

@@ -25,3 +25,18 @@ def test_queries_have_to_lie_in_their_memory():
     for stride in (width - 8, width + 4):
         with pytest.raises(KernelError, match="aligned"):
             K._kv4_queries("q", rows, stride, 2, width)
+
+
+def test_tables_and_batches_beyond_31_bits():
+    def of(*shape):
+        return torch.empty(shape, dtype=torch.int32, device="meta")
+
+    assert tuple(K._kv4_table("t", of(3, (1 << 31) - 1))) == (3, (1 << 31) - 1)
+    # the entry points take 32-bit sizes: 2^32 + 1 would come through as 1
+    for shape in ((1, 1 << 31), (1, (1 << 32) + 1), ((1 << 32) + 2, 1), ((1 << 31), 0)):
+        with pytest.raises(KernelError, match="block table"):
+            K._kv4_table("t", of(*shape))
+    K._kv4_rows("r", of(9), of(9), of((1 << 31) - 1), 9)
+    for n in (1 << 31, (1 << 32) + 1):
+        with pytest.raises(KernelError, match="slots"):
+            K._kv4_rows("r", of(9), of(9), of(n), 9)
