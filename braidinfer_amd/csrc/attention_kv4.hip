@@ -1,7 +1,7 @@
 // Attention over the cache of 4-bit keys and values (layout and number format: kv4.h), on the gfx950 matrix cores.
 //
-// Per (query row, kv head) the online softmax m' = max(m, s), c = 2^(m - m'), l = l c + p, o = o c + p v with scores in base 2
-// (scaled by scale * log2 e once), in float.  Codes become bfloat16 on their way into the matrix instructions: a code times its
+// Per (query row, kv head) the online softmax c = 2^(m - m'), l = l c + p, o = o c + p v, p = 2^(s - m') with scores in base 2
+// (scaled by scale * log2 e once) and m' no less than any of them, in float.  Codes become bfloat16 on their way into the matrix instructions: a code times its
 // scale is exact there, so keys, values and queries enter exactly and only the probabilities are rounded (to bfloat16, half a
 // step of 2^-8 each, which the sum over the keys averages; their sum l is taken of the rounded ones).  The instructions that take 4-bit operands with their scales as they
 // are would need the queries as two 8-bit parts, and add their products less exactly: up to 2e-5 of sum |q k| away for normal
@@ -16,6 +16,7 @@
 #include "prefill_order.h"
 
 #define LOG2E 1.4426950408889634f
+#define KV4_ABOVE 8.f
 __device__ __forceinline__ float kv4_exp2(float x) { return __builtin_amdgcn_exp2f(x); }
 
 __device__ __forceinline__ bf16x8 kv4_zero8() {
@@ -295,10 +296,11 @@ struct Kv4State {
 #pragma unroll
         for (int i = 1; i < OWN; ++i) mx = fmaxf(mx, fmaxf(fmaxf(t[i][0], t[i][1]), fmaxf(t[i][2], t[i][3])));
         mx *= scale2;                                                // the scale is positive
-        // The maximum that is subtracted need not be the largest score: weights up to 2^8 lose nothing in float or bfloat16.  So the
-        // lanes' maxima are brought together, and the sums rescaled, only when one is beyond that.
-        if (__any(mx > m + 8.f)) {
-            const float m_new = fmaxf(m, largest(mx));
+        // What is subtracted need not be the largest score: it is KV4_ABOVE powers of two beyond the largest one of the time it was chosen, and the
+        // lanes' maxima are brought together, and the sums rescaled, only when a score is beyond it.  Weights of 2^-KV4_ABOVE lose
+        // nothing in float or bfloat16, and none is above 1: sums of weights and values stay within what the values themselves reach.
+        if (__any(mx > m)) {
+            const float m_new = fmaxf(m, largest(mx) + KV4_ABOVE);
             const float corr = m_new == -INFINITY ? 1.f : kv4_exp2(m - m_new);
             m = m_new;
             l *= corr;
@@ -926,8 +928,8 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(NW == 4
 #pragma unroll
             for (int r = 3; r < 15; r += 2) mx = fmaxf(fmaxf(mx, s[r]), s[r + 1]);
             mx = fmaxf(mx, s[15]) * scale2;                                  // the scale is positive
-            if (__any(mx > m + 8.f)) {                                       // see Kv4State::weights
-                const float m_new = fmaxf(m, fmaxf(mx, __shfl_xor(mx, 32, WAVE)));
+            if (__any(mx > m)) {                                             // see Kv4State::weights
+                const float m_new = fmaxf(m, fmaxf(mx, __shfl_xor(mx, 32, WAVE)) + KV4_ABOVE);
                 const float corr = m_new == -INFINITY ? 1.f : kv4_exp2(m - m_new);
                 m = m_new;
                 l *= corr;

@@ -72,3 +72,23 @@ def test_rows_in_front_of_the_first_sequence_stay(nsplit):
         want, size, most = P.attention(q[at:at + n].astype(np.float64), k, v, 0.1, length - n)
         assert (np.abs(got[at:at + n] - want) <= tolerance(want, size, most, hd, length)).all()
         at += n
+
+
+@pytest.mark.parametrize("hd,nq", [(32, 4), (64, 8), (128, 4), (128, 16), (160, 3), (256, 12)])
+@pytest.mark.parametrize("nsplit", [1, 2, 64])
+def test_values_close_to_the_largest_number(hd, nq, nsplit):
+    """One token weighs 2^7 times as much as each of the others and its value is 6 x 2^125: a product of the two, as they are, is beyond what a
+    float holds, the result is not."""
+    n = 5 * PAGE + 9
+    c = Cache([n], 1, hd)
+    k, v = np.zeros((n, 1, hd)), np.zeros((n, 1, hd))
+    loud = n - 5
+    k[loud], v[loud] = 1.0, 6 * 2.0 ** 125
+    for p in range(n):
+        c.put(0, p, k[p], v[p])
+    scale = 7 * np.log(2) / hd
+    q = np.ones((4, nq, hd))
+    for got, first in ((decode(c, q[:1], None, scale, nsplit), n - 1), (prefill(c, q, [4], None, scale, nsplit), n - 4)):
+        want, size, most = P.attention(q[:len(got)], P.held(k), P.held(v), scale, first)
+        assert np.isfinite(got).all() and want.min() > 1e37
+        assert (np.abs(got - want) <= tolerance(want, size, most, hd, n)).all()
