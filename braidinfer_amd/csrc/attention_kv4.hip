@@ -1079,15 +1079,16 @@ extern "C" int br_attn_prefill_kv4(const void* q, size_t q_stride, void* out, co
     if (rows > 0x7fffffffLL - 256) return BR_BAD_ARG;
     if (B == 0 || max_new == 0) return BR_OK;
     // 8 waves convert a page once for 256 rows.  Tiles of 128 rows, two waves to 32 of them and each with a half of every page, where 256 would
-    // leave units without a tile or a few long ones last: 128 tokens of 32 heads of 128 over 8 in 11.0 us, not 13.3, 512 19.2 / 24.6, 2,048
-    // 66 / 74, but 3,000 126 / 102; for several sequences, whose tiles differ less, earlier: twice 1,500 79 / 70, 8 times 250 26 / 23.  Of heads
-    // of up to 64 two workgroups share a unit (32 over 4 heads of 64: 2,000 tokens 47.8 / 58.0, 1,357 to 93 50 / 52, 16 times 500 56 / 43, 8,192 387 / 332).
-    // In runs: 5 tokens behind 3,800 of 8 users 33 / 40, 16 behind 16,000 23.3 / 24.6, 32 behind 16,352 29.3 / 28.1.
+    // leave units without a tile or a few long ones last: 128 tokens of 32 heads of 128 over 8 in 10.7 us, not 13.1, 512 18.5 / 24.1, 2,048
+    // 62 / 72, but 3,000 122 / 99; for several sequences, whose tiles differ less, earlier: twice 1,500 75 / 54, 8 times 250 24.9 / 20.3.  Of heads
+    // of up to 64 two workgroups share a unit (32 over 4 heads of 64: 2,000 tokens 43.7 / 54.0, 16 times 500 51 / 38, 8,192 365 / 321; five of
+    // 1,357 to 93 have 128 rows by this rule, 45 / 41.5).
+    // In runs: 5 tokens behind 3,800 of 8 users 26.3 / 29.6, 16 behind 16,000 22.7 / 24.0, 32 behind 16,352 28.8 / 27.4.
     const int cus = br_device_cus() > 0 ? br_device_cus() : 256, each = hd <= 64 ? 2 : 1;
     const long long filled = ((long long)n_tokens * (nq / nkv) + 255) / 256 * nkv;
     // Heads beyond 128 have no registers for 256 rows, and from 8 waves of 256 channels 34 spill: two prompts of 158 and 109 tokens of 12 heads
-    // over 4 and 24 over 8 take 4 waves of 32 rows, each alone on its SIMD, 19.0 and 19.4 us, 8 waves 19.8 and 22.3; 1,646 tokens 66 / 60, 8,192 947 / 749 (of
-    // heads of 160 740 / 459).
+    // over 4 and 24 over 8 take 4 waves of 32 rows, each alone on its SIMD, 18.6 and 19.0 us, 8 waves 19.6 and 20.2; 1,646 tokens 65 / 59, 8,192 960 / 758 (of
+    // heads of 160 740 / 469).  Of heads of 64, four waves a SIMD with 128 registers each, 2 spill.
     const bool half = hd < 256 || nsplit > 1 || max_new > 256;
     const bool wide = hd <= 128 && (nsplit > 1 ? rows > 64 : filled > (each == 2 || B == 1 ? each * cus : cus / 2));
     const int most = wide ? 256 : 128;

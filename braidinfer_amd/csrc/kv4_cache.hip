@@ -106,7 +106,8 @@ __device__ __forceinline__ void kv4_rotate_pairs(T* row, const float* c, const f
 // they are held, as the cache of that type holds them.  The first `kv_blocks` columns of the grid take keys and values; the others
 // rotate the queries of the same 8 tokens where they stand.  A row and the look-up of its page are on their way together, and of 128
 // and 256 channels a lane loads both halves of its pairs once: what is moved bounds the launch (16,384 rows of 32 + 2 x 8 heads of 128
-// in 58.3 us, 6.2 TB/s of the bytes it has to move; 8 rows 3.4 us, which is what a launch and two dependent loads take).
+// in 68 us, 5.3 TB/s of the bytes it has to move, the rate of a copy; the same rows again and again, partly from the caches, 58; 8 rows 3.2
+// us, which is what a launch and two dependent loads take).
 template <typename T, int M, bool ROT>
 __global__ __launch_bounds__(256) void kv4_write_kernel(T* __restrict__ qkv, const float* __restrict__ cs, const float* __restrict__ sn,
                                                         Kv4Place place, unsigned char* __restrict__ cache, long long n_tokens, int nq,

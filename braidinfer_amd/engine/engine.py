@@ -102,7 +102,10 @@ class Engine:
                     use_graphs: bool = True, kv_cache: Optional[str] = None) -> "Engine":
         """A model folder (config.json and model.safetensors, or shards with their index).
         `kv_cache` "mxfp4" holds keys and values in 4 bits (bfloat16 models whose mixers are GQA attention with
-        heads in steps of 32): a quarter of the memory and of the bytes that attention reads; None: in `dtype`.
+        heads in steps of 32): a quarter of the memory and of the bytes that attention reads.  Single-token steps are faster
+        from there on where those bytes count (many sequences, or one of 16,000 tokens) and slower below (one of 1,000: a
+        tenth; writing is a launch of its own in every layer); normal rows are rounded by 0.115 of their root mean
+        square.  None: in `dtype`.
         `engine.load_profile.line()` says how the load went (the reference prints a
         `LOAD PROFILE` line, bin/generate.rs:62-68)."""
         config = config_from_folder(folder)

@@ -2042,11 +2042,12 @@ def attention_kv4_splits(n_seqs: int, max_new: int, nq: int, nkv: int, hd: int, 
     seen = max_ctx if window is None else min(max_ctx, window + max_new)
     pages = max(1, -(-seen // KV4_PAGE) + (window is not None))
     if decode if decode is not None else max_new == 1:
-        # One workgroup for a sequence and kv head takes 5 us and 0.4 for each page; cut into equal shares of all pages with a second
-        # launch that joins them, 11 us and the time of all bytes (8 kv heads of 128, both ways, us: one sequence of 700 tokens 8.3 / 12.3,
-        # 1,500 11.5 / 10.2; 8 of 128 to 2,048 15.9 / 13.6; 24 of 1,500 13.9 / 17.8; 32 of 128 to 8,192 52 / 38; 64 of 128 to 2,048 19.5 / 27.4,
-        # of 4,160 49 / 61, of 128 to 8,192 63 / 62; 16 of 32,768 194 / 99).  The more of them there are, the longer the one way stays
-        # ahead: the bytes of all then take their time either way.
+        # One workgroup for a sequence and kv head takes 5 us and 0.25 to 0.35 for each page; cut into equal shares of all pages with a second
+        # launch that joins them, 10 us and the time of all bytes (8 kv heads of 128, both ways, us: one sequence of 700 tokens 7.2 / 11.6,
+        # 1,088 10.4 / 11.6, 1,500 11.5 / 10.6, 2,000 12.1 / 10.2; 8 of 1,100 11.4 / 12.3, of 128 to 2,048 15.1 / 13.0; 24 of 1,500 14.0 / 17.2;
+        # 32 of 128 to 8,192 51.6 / 34.3; 64 of 128 to 2,048 20.8 / 26.4, of 4,160 50.6 / 57.2, of 128 to 8,192 62.9 / 57.2; 16 of 32,768
+        # 193 / 98).  The more of them there are, the longer the one way stays ahead: the bytes of all then take their time either
+        # way.  Bounds of contexts that are far from the contexts cost the difference: one of 700 in an engine of 8,192 tokens takes 11.6.
         heads = nq // nkv
         groups = n_seqs * nkv * -(-heads // (4 if heads <= 4 else 8 if heads <= 8 else 16))
         if pages <= min(80, 16 + groups // 8):
@@ -2055,10 +2056,10 @@ def attention_kv4_splits(n_seqs: int, max_new: int, nq: int, nkv: int, hd: int, 
         return max(2, min(64, -(-pages // 4) + 1, 2 + 24 * cus // max(1, groups)))
     # (The number above only bounds a sequence's pieces; here every row comes in as many.  One new token each behind 8 of 32,768 by this rule: 4 runs 151
     # us, where 64 are 221; four of 8,000, 4 kv heads of 64: 16 runs 19.3, 33 26.6.)
-    # Tiles of 256 rows (128 of heads beyond 128): as many runs at most as fill the compute units once (67 tokens behind 16,344: 608 us
-    # whole, 79 in 8 runs, 50 in 16, 73 in 20).  A page takes a run about `page` us, the join 7 with its launch and `run` for each run's sums (one kv head, 6
-    # and 128 tokens behind 2,048, us whole / in 4 / 16 / 32 runs: heads of 128 44 / 18 / 12.7 / 12.9 and 48 / 27 / 19 / 21, of 256 112 / 30 / 20 / 20
-    # and 118 / 39 / 28 / 31; a prompt of 1,024 through 8 kv heads 33 whole, 44 in 2).
+    # Tiles of 256 rows (128 of heads beyond 128): as many runs at most as fill the compute units once (67 tokens behind 16,344: 343 us
+    # whole, 75 in 8 runs, 48 in 16, 64 in 20).  A page takes a run about `page` us, the join 7 with its launch and `run` for each run's sums (one kv head, 6
+    # and 128 tokens behind 2,048, us whole / in 4 / 16 / 32 runs: heads of 128 44 / 18 / 12.9 / 13.1 and 49 / 28 / 20 / 22, of 256 113 / 31 / 21 / 22
+    # and 126 / 41 / 30 / 31; a prompt of 1,024 through 8 kv heads 32 whole, 41 in 2).
     rows, tile = max_new * (nq // nkv), 256 if hd <= 128 else 128
     groups = max(1, n_seqs * nkv * -(-rows // tile))
     if window is not None:                           # a tile's rows are of few tokens
@@ -2117,8 +2118,8 @@ def attention_decode_kv4(q: torch.Tensor, q_stride: int, out: torch.Tensor, slot
                          window: Optional[int], scale: float, nsplit: int, part_o: Optional[torch.Tensor] = None,
                          part_ml: Optional[torch.Tensor] = None) -> None:
     """`attention_decode_bf16` over a cache of 4-bit keys and values: one new token per sequence, which the cache holds
-    already (`rope_kv4_write`).  Rows of padding sequences, and of sequences of no tokens, are zero.  `nsplit`:
-    `attention_kv4_splits`.  Two calls that may run at the same time need scratch of their own."""
+    already (`rope_kv4_write`).  Rows of padding sequences, of sequences of no tokens, and rows all of whose scores are minus
+    infinity are zero.  `nsplit`: `attention_kv4_splits`.  Two calls that may run at the same time need scratch of their own."""
     name = "attention_decode_kv4"
     q_at, out_at, held, o_at, ml_at = _attention_kv4(name, q, q_stride, out, slots, ctx_lens, block_table, cache, B, B, nq, nkv, hd, page, window,
                                                      scale, nsplit, part_o, part_ml)
@@ -2135,7 +2136,7 @@ def attention_prefill_kv4(q: torch.Tensor, q_stride: int, out: torch.Tensor, cu_
                           part_o: Optional[torch.Tensor] = None, part_ml: Optional[torch.Tensor] = None) -> None:
     """`attention_prefill_bf16` over a cache of 4-bit keys and values, which holds the new tokens already (`rope_kv4_write`):
     sequence b's are rows cu_seqlens[b] .. cu_seqlens[b + 1] of `out` and `q`, the last of its ctx_lens[b] tokens; `max_new` is
-    the most of one sequence.  Rows of padding sequences are zero, rows in front of the first sequence and behind the last stay as they
+    the most of one sequence.  Rows of padding sequences, and rows all of whose scores are minus infinity, are zero, rows in front of the first sequence and behind the last stay as they
     are.  `nsplit`: `attention_kv4_splits`.  Two calls that may run at the same time need scratch of their own."""
     name = "attention_prefill_kv4"
     T = out.shape[0] if out.dim() == 2 else 0
